@@ -15,7 +15,10 @@ OBJDIR   := $(PKG)/build
 LIB      := $(PKG)/lib/libwhisper.so
 SFLIB    := $(PKG)/lib/libsortformer.so
 
-FLAGS    := -O3 -g -std=c++17 -fPIC -ffp-contract=off --offload-arch=$(ARCH) -Iinclude -I$(SRC) \
+# packed f32 instructions (v_pk_{add,mul,fma}_f32) are off: some of their forms have given wrong results
+# on this hardware now and then; the host pass warns that it does not know the feature (harmless)
+NOPK     := -Xclang -target-feature -Xclang -packed-fp32-ops
+FLAGS    := -O3 -g -std=c++17 -fPIC -ffp-contract=off --offload-arch=$(ARCH) $(NOPK) -Iinclude -I$(SRC) \
             -DWHISPER_SHARED -DWHISPER_BUILD -Wall -Wno-unused-function -Wno-unused-variable
 
 HIP_SRCS := $(wildcard $(SRC)/*.hip)

@@ -91,12 +91,12 @@ class FullExt(C.Structure):
     _fields_ = [("suppress_eot", C.c_int), ("samples_on_device", C.c_int), ("reserved", C.c_int * 6)]
 
 
-# every symbol include/whisper.h + include/owk.h declare (checked by tests/test_abi.py)
+# every symbol include/whisper.h + include/owk*.h declare (checked by tests/test_abi.py)
 def header_symbols(include_dir=None):
     import re
     include_dir = include_dir or os.path.normpath(os.path.join(HERE, "..", "..", "include"))
     syms = []
-    for h in ("whisper.h", "owk.h", "owk_diarize.h", "ggml-backend.h"):
+    for h in ("whisper.h", "owk.h", "owk_diarize.h", "owk_kv8.h", "ggml-backend.h"):
         txt = open(os.path.join(include_dir, h)).read()
         txt = re.sub(r"/\*.*?\*/", "", txt, flags=re.S)
         for m in re.finditer(r"\b((?:whisper|owk|ggml_backend)_[a-z0-9_]+)\s*\(", txt):

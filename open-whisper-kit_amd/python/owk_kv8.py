@@ -1,0 +1,205 @@
+"""Binding of include/owk_kv8.h: keys and values held in 8 bits, on torch tensors of one GPU.
+
+    cache = Cache(n_seqs=4, n_heads=8, head_dim=64, max_tokens=4096, device="cuda")
+    cache.append(k, v, lens)                    # k, v: [4, n, 8, 64], their tokens go behind lens[b]
+    out = cache.attend(q, lens, causal=True)    # q: [4, n, 8 * group, 64] -> the same shape
+    lens += n
+
+Tensors of entries are padded, [entry, row, head, head_dim] with `count` rows each (None: all), or joined,
+[row, head, head_dim] with entry b's rows at off[b] .. off[b + 1] - 1; the innermost dimension is contiguous.
+Index tensors (lens, seq, off, count, first) are int32 on the cache's device and are read there: nothing
+here waits for the GPU, and every call can be captured into a graph. Calls go to the current stream of
+the cache's device. One layer of a model is one Cache; layers share lens. Bad arguments raise ValueError.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch  # before the library: both use one HIP runtime
+
+import owk
+
+BLOCK = 64
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+class CacheDesc(C.Structure):
+    _fields_ = [("device", C.c_int), ("dtype", C.c_int), ("head_dim", C.c_int), ("n_heads", C.c_int), ("n_seqs", C.c_int),
+                ("n_blocks", C.c_int), ("max_blocks", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("k_tail", C.c_void_p), ("v_tail", C.c_void_p),
+                ("table", C.c_void_p)]
+
+
+class Batch(C.Structure):
+    _fields_ = [("n", C.c_int), ("max_new", C.c_int), ("rows", C.c_int64), ("lens", C.c_void_p), ("seq", C.c_void_p),
+                ("off", C.c_void_p), ("count", C.c_void_p)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("entry", C.c_int64), ("row", C.c_int64), ("head", C.c_int64)]
+
+
+class AttendParams(C.Structure):
+    _fields_ = [("n_q_heads", C.c_int), ("causal", C.c_int), ("out_type", C.c_int), ("max_len", C.c_int), ("scale", C.c_float)]
+
+
+_lib = None
+
+
+def load():
+    global _lib
+    if _lib is None:
+        L = owk.load()
+        cp, bp, rp, ap, vp = (C.POINTER(t) for t in (CacheDesc, Batch, Rows, AttendParams, C.c_char))
+        vp = C.c_void_p
+        L.owk_kv8_append.argtypes = [cp, bp, rp, rp, vp]
+        L.owk_kv8_attend.argtypes = [cp, bp, ap, rp, rp, vp, C.c_size_t, vp]
+        L.owk_kv8_attend_workspace.argtypes = [cp, bp, ap]
+        L.owk_kv8_attend_workspace.restype = C.c_size_t
+        L.owk_kv8_read.argtypes = [cp, C.c_int, C.c_int, vp, vp, vp, rp, rp, vp]
+        L.owk_kv8_error.restype = C.c_char_p
+        _lib = L
+    return _lib
+
+
+def _check(rc):
+    if rc:
+        msg = load().owk_kv8_error().decode("utf-8", "replace")
+        raise ValueError(msg) if rc == -1 else RuntimeError(msg)
+
+
+class Cache:
+    """The cache of one layer: `n_seqs` sequences of up to `max_tokens` tokens (rounded up to whole blocks). With
+    `table` (int32 [n_seqs, blocks], kept, read at every call) sequences take their blocks from a pool of `n_blocks`."""
+
+    def __init__(self, n_seqs, n_heads, head_dim, max_tokens, dtype=torch.float16, device="cuda", n_blocks=None, table=None):
+        blocks = table.shape[1] if table is not None else -(-int(max_tokens) // BLOCK)
+        pool = n_blocks if n_blocks is not None else n_seqs * blocks
+
+        def new(shape, t):
+            return torch.zeros(shape, dtype=t, device=device)
+
+        self._bind(new((pool, n_heads, BLOCK, head_dim), torch.int8), new((pool, n_heads, head_dim, BLOCK), torch.int8),
+                   new((pool, n_heads), torch.float32), new((pool, n_heads), torch.float32),
+                   new((n_seqs, n_heads, BLOCK, head_dim), dtype), new((n_seqs, n_heads, head_dim, BLOCK), dtype), table, blocks)
+
+    @classmethod
+    def of(cls, k, v, k_scale, v_scale, k_tail, v_tail, table=None, max_blocks=None):
+        """A cache over tensors that the caller made, in the layouts of owk_kv8.h. Without a table the pool is cut into
+        equal runs of `max_blocks` blocks (None: as many as fit)."""
+        self = cls.__new__(cls)
+        blocks = table.shape[1] if table is not None else max_blocks or k.shape[0] // max(1, k_tail.shape[0])
+        self._bind(k, v, k_scale, v_scale, k_tail, v_tail, table, blocks)
+        return self
+
+    def _bind(self, k, v, k_scale, v_scale, k_tail, v_tail, table, blocks):
+        pool, heads, _, dim = k.shape
+        seqs, dtype, dev = k_tail.shape[0], k_tail.dtype, k.device
+        want = ((k, torch.int8, (pool, heads, BLOCK, dim)), (v, torch.int8, (pool, heads, dim, BLOCK)),
+                (k_scale, torch.float32, (pool, heads)), (v_scale, torch.float32, (pool, heads)),
+                (k_tail, dtype, (seqs, heads, BLOCK, dim)), (v_tail, dtype, (seqs, heads, dim, BLOCK)))
+        for x, t, shape in want + (((table, torch.int32, (seqs, blocks)),) if table is not None else ()):
+            if x.dtype != t or tuple(x.shape) != shape or x.device != dev or not x.is_contiguous():
+                raise ValueError(f"a cache tensor is {x.dtype} {tuple(x.shape)} on {x.device}, wanted contiguous {t} {shape} on {dev}")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"a cache of {dtype}: float16 or bfloat16 are supported")
+        if dim not in (64, 128):
+            raise ValueError(f"head_dim {dim}: 64 or 128 are supported")
+        if dev.type != "cuda":
+            raise ValueError(f"the cache is on {dev}: a GPU is needed")
+        if table is None and not 0 < seqs * blocks <= pool:
+            raise ValueError(f"{seqs} sequences of {blocks} blocks do not fit a pool of {pool}")
+        self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.table = (
+            k, v, k_scale, v_scale, k_tail, v_tail, table)
+        self.device, self.dtype, self.n_heads, self.head_dim = dev, dtype, heads, dim
+        self.n_seqs, self.max_tokens = seqs, blocks * BLOCK
+        self.desc = CacheDesc(dev.index, _TYPES[dtype], dim, heads, seqs, pool, blocks, k.data_ptr(), v.data_ptr(),
+                              k_scale.data_ptr(), v_scale.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(),
+                              table.data_ptr() if table is not None else None)
+        self._ref = C.byref(self.desc)
+        self._L = load()
+
+    def _index(self, name, x, n):
+        if x is None:
+            return None
+        if x.dtype != torch.int32 or x.device != self.device or x.dim() != 1 or x.shape[0] != n or not x.is_contiguous():
+            raise ValueError(f"{name} is {x.dtype} {tuple(x.shape)} on {x.device}, wanted contiguous int32 ({n},) on {self.device}")
+        return x.data_ptr()
+
+    def _batch(self, x, lens, seq, off, count, max_new):
+        n = lens.shape[0]
+        if off is None:
+            if x.dim() != 4 or x.shape[0] != n:
+                raise ValueError(f"a padded tensor of {n} entries is [{n}, rows, heads, {self.head_dim}], got {tuple(x.shape)}")
+            most = x.shape[1]
+            if max_new is not None and max_new > most:
+                raise ValueError(f"max_new {max_new} passes the tensor's {most} rows")
+            return Batch(n, most if max_new is None else max_new, 0, self._index("lens", lens, n),
+                         self._index("seq", self._seq(seq, n), n), None, self._index("count", count, n))
+        if x.dim() != 3 or count is not None:
+            raise ValueError(f"joined tensors are [rows, heads, {self.head_dim}] without count, got {tuple(x.shape)}")
+        rows = x.shape[0]
+        return Batch(n, rows if max_new is None else max_new, rows, self._index("lens", lens, n),
+                     self._index("seq", self._seq(seq, n), n), self._index("off", off, n + 1), None)
+
+    def _seq(self, seq, n):
+        if seq is None and n > self.n_seqs:
+            raise ValueError(f"{n} entries, and the cache has {self.n_seqs} sequences")
+        return seq
+
+    def _rows(self, name, x, heads, dtype):
+        if x.dtype != dtype or x.device != self.device or x.shape[-1] != self.head_dim or (heads and x.shape[-2] != heads):
+            raise ValueError(f"{name} is {x.dtype} {tuple(x.shape)} on {x.device}, wanted {dtype} [.., {heads or 'heads'}, "
+                             f"{self.head_dim}] on {self.device}")
+        s = x.stride()
+        if s[-1] != 1:
+            raise ValueError(f"the innermost dimension of {name} is not contiguous")
+        return Rows(x.data_ptr(), s[0] if x.dim() == 4 else 0, s[-3], s[-2])
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def append(self, k, v, lens, seq=None, off=None, count=None, max_new=None):
+        """Store the entries' tokens behind the lens[b] that their sequences hold (or from an earlier multiple of 64 on)."""
+        b = self._batch(k, lens, seq, off, count, max_new)
+        if k.shape != v.shape:
+            raise ValueError(f"k is {tuple(k.shape)} and v is {tuple(v.shape)}")
+        kr, vr = self._rows("k", k, self.n_heads, self.dtype), self._rows("v", v, self.n_heads, self.dtype)
+        if k.numel():
+            _check(self._L.owk_kv8_append(self._ref, b, kr, vr, self._stream()))
+
+    def attend(self, q, lens, seq=None, off=None, count=None, max_new=None, max_len=0, scale=None, causal=False, out=None):
+        """softmax(scale * q . k) . v over what the sequences hold: tokens [0, lens[b]), or with causal, for row i,
+        [0, lens[b] + i] (its own tokens appended before). scale None: 1 / sqrt(head_dim). `max_len`: no sequence holds
+        more (a hint for splitting the work). `out`: a tensor like q, or float32; rows that are no entry's stay as they are."""
+        b = self._batch(q, lens, seq, off, count, max_new)
+        heads = q.shape[-2]
+        qr = self._rows("q", q, 0, self.dtype)
+        if heads < 1 or heads % self.n_heads:
+            raise ValueError(f"{heads} query heads are no multiple of {self.n_heads} key/value heads")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape:
+            raise ValueError(f"out is {tuple(out.shape)} and q is {tuple(q.shape)}")
+        elif any(n > 1 and t == 0 for n, t in zip(out.shape, out.stride())):
+            raise ValueError("rows of out lie on each other")
+        p = AttendParams(heads, 1 if causal else 0, _TYPES.get(out.dtype, -1), max_len,
+                         self.head_dim ** -0.5 if scale is None else scale)
+        orow = self._rows("out", out, heads, torch.float32 if out.dtype == torch.float32 else self.dtype)
+        if q.numel():
+            n = self._L.owk_kv8_attend_workspace(self._ref, b, p)
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+            _check(self._L.owk_kv8_attend(self._ref, b, p, qr, orow, ws.data_ptr() if n else None, n, self._stream()))
+        return out
+
+    def read(self, lens, max_tokens, seq=None, first=None):
+        """Tokens first[b] (None: 0) .. + max_tokens of sequences that hold lens[b]: (k, v), each [entry, token, head,
+        head_dim] in the cache's 16-bit type, zeros from lens[b] on."""
+        n = lens.shape[0]
+        k = torch.empty((n, max_tokens, self.n_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        v = torch.empty_like(k)
+        i = [self._index("lens", lens, n), self._index("seq", self._seq(seq, n), n), self._index("first", first, n)]
+        if k.numel():
+            _check(self._L.owk_kv8_read(self._ref, n, max_tokens, *i, self._rows("k", k, 0, self.dtype),
+                                        self._rows("v", v, 0, self.dtype), self._stream()))
+        return k, v

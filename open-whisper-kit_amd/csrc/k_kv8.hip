@@ -4,6 +4,9 @@
 // Codes of keys lie token-major [64][D], codes of values dimension-major [D][64]: each is then the
 // operand that its matrix product reads along its sum (keys along D, values along the tokens), 16
 // contiguous bytes a lane. The incomplete last block (tail) lies in 16 bits in the same two orders.
+#include <algorithm>
+#include <climits>
+
 #include "kv8.h"
 
 namespace owk {
@@ -11,6 +14,8 @@ namespace owk {
 namespace {
 
 typedef __bf16 bf16_t;
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int BLK = kKv8Block;
@@ -185,81 +190,352 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Call a, const int32_t * fir
 }
 
 // ---------------------------------------------------------------------------------------------------
-// attend
+// attend, few rows
 // ---------------------------------------------------------------------------------------------------
-// One workgroup per (row, query head, entry): wave w takes blocks w, w + 4, ..; a lane is a key while
-// scores are made and a dimension while values are added.
-template <typename T, int D, typename O>
-__global__ __launch_bounds__(256) void k_kv8_attend(Kv8Call a, Kv8Attend p) {
-    constexpr int DL = D / 64;  // dimensions of a lane
-    const int b = blockIdx.z, qh = blockIdx.y, i = blockIdx.x, head = qh / p.group;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+// A tile is 16 rows of one entry and key/value head: row r of the entry's n * group is query row r / group,
+// query head head * group + r % group. A wave takes every W-th block of 64 keys, straight from memory into
+// registers (each byte of the cache is read once a tile, so there is nothing to stage), and keeps a running
+// maximum m, sum l and accumulator of its own; the waves are joined in a fixed order at the end.
+//
+// Both products run on the codes themselves (16x16x64 i8 -> i32, exact): no code is ever converted. What
+// meets them is fixed point in two signed digits of 7 bits, value = unit * (128 * hi + lo):
+//   queries         unit = max|q| of the row / 16255: off by at most max|q| * 2^-15
+//   probabilities   exp2(s - block's maximum) in (0, 1], unit 1 / 16256: off by at most 2^-15 of the block's largest
+// The scale of a block multiplies the finished integer sums, in f32.
+//
+// Lanes: c = lane & 15 is the row (a column of S^T = K Q^T and of O^T = V^T P^T), g = lane >> 4. Key tile t
+// feeds key 16 (m >> 2) + 4 t + (m & 3) as row m, so lane (c, g) ends up with the scores of keys 16 g .. 16 g + 15
+// in order: exactly the 16 bytes of P^T that the second product wants of it. Nothing crosses lanes but the maximum.
+constexpr float QUNIT = 16255.0f, PUNIT = 16256.0f;
+constexpr float LOG2E = 1.44269504088896340736f;
+
+__device__ __forceinline__ float max_over_g(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ int max_over_g(int x) {
+    x = max(x, __shfl_xor(x, 16));
+    return max(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_over_g(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// the two digits of 16 values in [0, 16256], a byte each
+__device__ __forceinline__ void digits(const float (&p)[4][4], i32x4 & hi, i32x4 & lo) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        uint32_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (uint32_t) fmaf(p[t][i], PUNIT, 0.5f);
+        const uint32_t a = x[0] | x[1] << 16, b = x[2] | x[3] << 16;
+        hi[t] = __builtin_amdgcn_perm(b >> 7, a >> 7, 0x06040200);
+        lo[t] = __builtin_amdgcn_perm(b, a, 0x06040200) & 0x7f7f7f7f;
+    }
+}
+
+// a wave's state for its 16 rows
+template <int D> struct Acc {
+    float m = -INFINITY, l = 0.0f;  // m in units of log2, the same in all four lanes of a row; l a quarter
+    float o[D / 16][4];             // dimension 16 dt + 4 g + i
+    __device__ Acc() {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+    }
+    // what a block brings has its own maximum mb (-inf: nothing of it is seen): the factor of its sums
+    __device__ __forceinline__ float merge(float mb, float & alpha) {
+        const float top = fmaxf(m, mb);
+        alpha = m == -INFINITY ? 0.0f : exp2f(m - top);
+        const float f = mb == -INFINITY ? 0.0f : exp2f(mb - top);
+        m = top;
+        l *= alpha;
+        return f;
+    }
+};
+
+// the tail of a sequence: the same tile on 16x16x32 products of the tail's own 16-bit type, with f32 sums. Half-precision
+// probabilities are held times 2^14 (small ones stay normal), bf16 ones as a sum of two. A token whose values are not all
+// finite makes the rows that see it NaN and touches no other.
+__device__ __forceinline__ floatx4 mfma16(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+template <typename T, int D>
+__device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T * qrow, bool qvec, float unit, int have, int see,
+                                            Acc<D> & acc) {
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+    constexpr bool BF = !std::is_same<T, _Float16>::value;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    float s[4][4];
+    {
+        vec8 q[D / 32];
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            T x[8] = {};
+            if (qrow) load_row<T, 8>(qrow + j * 32 + g * 8, qvec, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[j][i] = x[i];
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int key = 16 * (c >> 2) + 4 * t + (c & 3);
+            floatx4 x = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                vec8 k = {};
+                if (key < have) k = *(const vec8 *) (kt + key * D + j * 32 + g * 8);
+                x = mfma16(k, q[j], x);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = x[i];
+        }
+    }
+    float mb = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[t][i] = 16 * g + 4 * t + i < see ? s[t][i] * unit : -INFINITY;
+            mb = fmaxf(mb, s[t][i]);
+        }
+    mb = max_over_g(mb);
+    float alpha;
+    const float f = acc.merge(mb, alpha);
+    const float base = mb == -INFINITY ? 0.0f : mb;  // a NaN score is in no maximum, and makes its probability NaN
+    float ls = 0.0f;
+    vec8 ph[2], pl[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p = exp2f(s[t][i] - base);
+            ls += p;
+            const int k = t >> 1, e = 4 * (t & 1) + i;
+            ph[k][e] = (T) (BF ? p : p * 16384.0f);
+            if (BF) pl[k][e] = (T) (p - to_f32(ph[k][e]));
+        }
+    uint32_t bad = 0;  // of the lane's 16 keys
+    const float fo = BF ? f : f * (1.0f / 16384.0f);
+    // values, dimension-major: lane (c, g) reads keys 16 g .. 16 g + 15 of dimension 16 dt + c
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+        floatx4 x = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            vec8 v = *(const vec8 *) (vt + (dt * 16 + c) * BLK + 16 * g + 8 * k);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool mine = 16 * g + 8 * k + i < have, fine = finite(to_f32(v[i]));
+                bad |= mine && !fine ? 1u << (8 * k + i) : 0u;
+                v[i] = mine && fine ? v[i] : (T) 0.0f;
+            }
+            x = mfma16(v, ph[k], x);
+            if (BF) x = mfma16(v, pl[k], x);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc.o[dt][i] = fmaf(x[i], fo, acc.o[dt][i] * alpha);
+    }
+    if (__any(bad != 0)) {
+        for (int o = 8; o; o >>= 1) bad |= __shfl_xor(bad, o);  // over c: the keys of group g
+        const int n = min(max(see - 16 * g, 0), 16);
+        if (bad & ((1u << n) - 1)) ls = NAN;
+    }
+    acc.l += f * ls;
+}
+
+template <typename T, int D, typename O, int W>
+__global__ __launch_bounds__(W * 64) void k_kv8_attend_rows(Kv8Call a, Kv8Attend p) {
+    constexpr int DT = D / 16, KC = D / 64;
+    const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, head = blockIdx.y, b = blockIdx.z;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const Kv8Entry e = kv8_entry(a, b);
-    if (i >= e.n) return;
+    const int rows = e.n * p.group - tile * 16;  // of this tile, and of those behind it
+    if (rows <= 0) return;
     const int cap = a.c.max_blocks * BLK;
     const int stored = e.seq < 0 ? 0 : p.causal ? min(e.start + e.n, cap) : e.start;
-    const int seen = min(stored, p.causal ? e.start + i + 1 : stored);
-    __shared__ float q[D];
-    __shared__ float part[4][D + 2];
-    const T * qr = (const T *) row_at(a, p.q, e, b, i, qh, 2);
-    for (int d = threadIdx.x; d < D; d += 256) q[d] = to_f32(qr[d]) * p.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, acc[DL] = {};
-    for (int blk = w; blk * BLK < seen; blk += 4) {
-        const bool in_tail = blk == stored / BLK;
+    const int full = stored / BLK;
+    // what this lane's row sees, and what the tile sees at most
+    const int r = tile * 16 + c, qi = r / p.group;
+    const int see = p.causal ? min(stored, e.start + qi + 1) : stored;
+    const int last = min(tile * 16 + 15, e.n * p.group - 1) / p.group;
+    const int most = p.causal ? min(stored, e.start + last + 1) : stored;
+    const int first = p.causal ? min(stored, e.start + tile * 16 / p.group + 1) : stored;  // the least a row of it sees
+    const int blocks = (most + BLK - 1) / BLK, per = (blocks + p.splits - 1) / p.splits;
+    const int lo = split * per, hi = min(blocks, lo + per);
+
+    const T * qrow = c < rows ? (const T *) row_at(a, p.q, e, b, qi, head * p.group + r % p.group, 2) : nullptr;
+    const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
+    i32x4 qh[KC], ql[KC];
+    float qunit;
+    {
+        T x[KC][16];
+        float top = 0.0f;
+        bool ok = true;
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            if (qrow) load_row<T, 16>(qrow + k * 64 + g * 16, p.q.vec, x[k]);
+            else
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[k][i] = (T) 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float y = fabsf(to_f32(x[k][i]));
+                ok &= finite(y);
+                top = fmaxf(top, y);
+            }
+        }
+        top = max_over_g(ok ? top : INFINITY);
+        const float inv = finite(top) && top > 0.0f ? QUNIT / top : 0.0f;
+        // a row whose largest element is so small that QUNIT / top overflows counts as zeros
+        qunit = finite(top) ? (finite(inv) ? top / QUNIT : 0.0f) * fabsf(p.scale) * LOG2E : NAN;
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t h = 0, l = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int y = finite(inv) ? (int) rintf(to_f32(x[k][4 * j + i]) * inv * sgn) : 0;
+                    const int yh = (y + 64) >> 7;
+                    h |= (uint32_t) (yh & 255) << 8 * i;
+                    l |= (uint32_t) ((y - 128 * yh) & 255) << 8 * i;
+                }
+                qh[k][j] = h;
+                ql[k][j] = l;
+            }
+    }
+
+    Acc<D> acc;
+    for (int blk = lo + w; blk < hi; blk += W) {
+        if (blk == full) {
+            const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
+            attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qrow, p.q.vec, p.scale * LOG2E,
+                              stored - full * BLK, see - full * BLK, acc);
+            continue;
+        }
         const int64_t page = kv8_page(a.c, e.seq, blk);
-        if (!in_tail && page < 0) continue;
-        const int64_t hk = (page * a.c.n_heads + head);
-        const int64_t tk = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
-        const bool visible = blk * BLK + lane < seen;
-        float s = 0.0f;
-        if (visible) {
-            if (in_tail) {
-                const T * k = (const T *) a.c.k_tail + tk + lane * D;
-                for (int d = 0; d < D; ++d) s = fmaf(q[d], to_f32(k[d]), s);
-            } else {
-                const int8_t * k = a.c.k + hk * BLK * D + lane * D;
-                for (int d = 0; d < D; ++d) s = fmaf(q[d], (float) k[d], s);
-                s *= a.c.k_scale[hk];
-            }
-        }
-        const bool odd = __any(visible && !(s == s));
-        const float top = fmaxf(m, wave_max(visible ? s : -INFINITY));
-        const float base = top == -INFINITY ? 0.0f : top;
-        const float alpha = expf(m - base);
-        const float pr = odd ? NAN : visible ? expf(s - base) : 0.0f;
-        l = l * alpha + wave_sum(pr);
-        m = top;
+        if (page < 0) continue;
+        const int64_t at = page * a.c.n_heads + head;
+        const int8_t * kc = a.c.k + at * BLK * D;
+        const int8_t * vc = a.c.v + at * BLK * D;
+        i32x4 kx[4][KC], vx[DT];
 #pragma unroll
-        for (int g = 0; g < DL; ++g) {
-            const int d = g * 64 + lane;
-            float sum = 0.0f;
-            for (int t = 0; t < BLK; ++t) {
-                const float pt = __shfl(pr, t);
-                if (blk * BLK + t >= seen) continue;
-                const float v = in_tail ? to_f32(((const T *) a.c.v_tail + tk)[d * BLK + t]) : (float) (a.c.v + hk * BLK * D)[d * BLK + t];
-                sum = fmaf(pt, v, sum);
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int k = 0; k < KC; ++k) kx[t][k] = *(const i32x4 *) (kc + (16 * (c >> 2) + 4 * t + (c & 3)) * D + k * 64 + g * 16);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) vx[dt] = *(const i32x4 *) (vc + (dt * 16 + c) * BLK + g * 16);
+        const float f = qunit * a.c.k_scale[at], sv = a.c.v_scale[at];
+
+        int s[4][4], top = INT_MIN;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            i32x4 xh = {0, 0, 0, 0}, xl = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                xh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kx[t][k], qh[k], xh, 0, 0, 0);
+                xl = __builtin_amdgcn_mfma_i32_16x16x64_i8(kx[t][k], ql[k], xl, 0, 0, 0);
             }
-            acc[g] = acc[g] * alpha + (in_tail ? sum : sum * a.c.v_scale[hk]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = xh[i] * 128 + xl[i];
+        }
+        const int here = see - blk * BLK;
+        if (first < blk * BLK + BLK) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][i] = 16 * g + 4 * t + i < here ? s[t][i] : INT_MIN;
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, s[t][i]);
+        top = max_over_g(top);
+        const bool none = here <= 0;  // this row sees nothing of the block
+        const float mb = none ? -INFINITY : (float) top * f;
+        float alpha;
+        const float fb = acc.merge(mb, alpha);
+        float pr[4][4], ls = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // the difference of the integers is exact
+                pr[t][i] = s[t][i] == INT_MIN ? 0.0f : __builtin_amdgcn_exp2f((float) (s[t][i] - top) * f);
+                ls += pr[t][i];
+            }
+        acc.l += none ? 0.0f : fb * ls;
+        i32x4 ph, pl;
+        digits(pr, ph, pl);
+        const float fo = none ? 0.0f : fb * sv * (1.0f / PUNIT);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const i32x4 z = {0, 0, 0, 0};
+            const i32x4 xh = __builtin_amdgcn_mfma_i32_16x16x64_i8(vx[dt], ph, z, 0, 0, 0);
+            const i32x4 xl = __builtin_amdgcn_mfma_i32_16x16x64_i8(vx[dt], pl, z, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc.o[dt][i] = fmaf((float) (xh[i] * 128 + xl[i]), fo, acc.o[dt][i] * alpha);
         }
     }
-    if (lane == 0) {
-        part[w][D] = m;
-        part[w][D + 1] = l;
-    }
+
+    // join the waves, in order
+    __shared__ float ml[W][16][2];
+    __shared__ __align__(16) float o[W][16][D];
+    const float l = sum_over_g(acc.l);
+    if (c < rows) {
+        if (g == 0) {
+            ml[w][c][0] = acc.m;
+            ml[w][c][1] = l;
+        }
 #pragma unroll
-    for (int g = 0; g < DL; ++g) part[w][g * 64 + lane] = acc[g];
+        for (int dt = 0; dt < DT; ++dt) *(floatx4 *) &o[w][c][dt * 16 + 4 * g] = floatx4{acc.o[dt][0], acc.o[dt][1], acc.o[dt][2], acc.o[dt][3]};
+    }
     __syncthreads();
-    const float top = fmaxf(fmaxf(part[0][D], part[1][D]), fmaxf(part[2][D], part[3][D]));
-    const float base = top == -INFINITY ? 0.0f : top;
-    for (int d = threadIdx.x; d < D; d += 256) {
-        float o = 0.0f, total = 0.0f;
-        for (int k = 0; k < 4; ++k) {
-            const float f = expf(part[k][D] - base);
-            total += part[k][D + 1] * f;
-            o += part[k][d] * f;
+    const int n = min(rows, 16);
+    float * ws = p.ws + ((((int64_t) b * a.c.n_heads + head) * (gridDim.x / p.splits) + tile) * p.splits + split) * 16 * (D + 2);
+    for (int i = threadIdx.x; i < n * D; i += W * 64) {
+        const int row = i / D, d = i % D;
+        float top = -INFINITY, sum = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) top = fmaxf(top, ml[k][row][0]);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float f = ml[k][row][0] == -INFINITY ? 0.0f : exp2f(ml[k][row][0] - top);
+            // (a NaN maximum is in no fmaxf: its wave's l is NaN and is kept)
+            sum += f * ml[k][row][1] + (ml[k][row][1] == ml[k][row][1] ? 0.0f : NAN);
+            x += f * o[k][row][d];
         }
-        ((O *) row_at(a, p.out, e, b, i, qh, sizeof(O)))[d] = (O) (total == 0.0f ? 0.0f : o / total);
+        if (p.splits > 1) {
+            ws[row * (D + 2) + 2 + d] = x;
+            if (d < 2) ws[row * (D + 2) + d] = d ? sum : top;
+        } else {
+            const int q = tile * 16 + row;
+            ((O *) row_at(a, p.out, e, b, q / p.group, head * p.group + q % p.group, sizeof(O)))[d] = (O) (sum == 0.0f ? 0.0f : x / sum);
+        }
+    }
+}
+
+// joins the splits of a tile, in order
+template <int D, typename O> __global__ __launch_bounds__(256) void k_kv8_attend_join(Kv8Call a, Kv8Attend p) {
+    const int tile = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
+    const Kv8Entry e = kv8_entry(a, b);
+    const int n = min(e.n * p.group - tile * 16, 16);
+    const float * ws = p.ws + (((int64_t) b * a.c.n_heads + head) * gridDim.x + tile) * p.splits * 16 * (D + 2);
+    for (int i = threadIdx.x; i < n * D; i += 256) {
+        const int row = i / D, d = i % D;
+        float top = -INFINITY, sum = 0.0f, x = 0.0f;
+        for (int k = 0; k < p.splits; ++k) top = fmaxf(top, ws[(k * 16 + row) * (D + 2)]);
+        for (int k = 0; k < p.splits; ++k) {
+            const float * y = ws + (k * 16 + row) * (D + 2);
+            const float f = y[0] == -INFINITY ? 0.0f : exp2f(y[0] - top);
+            sum += f * y[1] + (y[1] == y[1] ? 0.0f : NAN);
+            x += f * y[2 + d];
+        }
+        const int q = tile * 16 + row;
+        ((O *) row_at(a, p.out, e, b, q / p.group, head * p.group + q % p.group, sizeof(O)))[d] = (O) (sum == 0.0f ? 0.0f : x / sum);
     }
 }
 
@@ -292,15 +568,34 @@ void kv8_read(hipStream_t s, const Kv8Call & call, const int32_t * first, const 
     });
 }
 
-Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) { return Kv8Plan{1, 0}; }
+// Splits: enough workgroups to fill the card, but no more than leaves a wave a block of its own
+Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) {
+    const int64_t tiles = ((int64_t) call.b.max_new * group + 15) / 16;
+    const int64_t groups = tiles * call.c.n_heads * call.b.n;
+    const int64_t blocks = (max_len + BLK - 1) / BLK;
+    int64_t splits = 1;
+    if (groups < 512) splits = std::min((1024 + groups - 1) / groups, (blocks + 3) / 4);
+    if (blocks <= 32) splits = 1;
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, 256));
+    Kv8Plan plan;
+    plan.splits = (int) splits;
+    plan.ws_bytes = splits > 1 ? (size_t) (groups * splits * 16 * (call.c.head_dim + 2)) * 4 : 0;
+    return plan;
+}
 
 void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, int out_type) {
-    const dim3 grid(call.b.max_new, call.c.n_heads * a.group, call.b.n);
+    const int tiles = (int) (((int64_t) call.b.max_new * a.group + 15) / 16);
+    const dim3 grid(tiles * a.splits, call.c.n_heads, call.b.n), join(tiles, call.c.n_heads, call.b.n);
     with_type(call.c, [&](auto t, auto d) {
         using T = decltype(t);
         constexpr int D = decltype(d)::value;
-        if (out_type == OWK_KV8_F32) OWK_LAUNCH((k_kv8_attend<T, D, float>), grid, dim3(256), 0, s, call, a);
-        else OWK_LAUNCH((k_kv8_attend<T, D, T>), grid, dim3(256), 0, s, call, a);
+        if (out_type == OWK_KV8_F32) {
+            OWK_LAUNCH((k_kv8_attend_rows<T, D, float, 4>), grid, dim3(256), 0, s, call, a);
+            if (a.splits > 1) OWK_LAUNCH((k_kv8_attend_join<D, float>), join, dim3(256), 0, s, call, a);
+        } else {
+            OWK_LAUNCH((k_kv8_attend_rows<T, D, T, 4>), grid, dim3(256), 0, s, call, a);
+            if (a.splits > 1) OWK_LAUNCH((k_kv8_attend_join<D, T>), join, dim3(256), 0, s, call, a);
+        }
     });
 }
 

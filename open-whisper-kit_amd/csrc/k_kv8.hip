@@ -150,30 +150,29 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8Call a, Kv8Rows kr, Kv8Ro
 // ---------------------------------------------------------------------------------------------------
 // read
 // ---------------------------------------------------------------------------------------------------
-// One workgroup per (block of the sequence, head, keys or values, entry), four threads a token.
+// One workgroup per (block of the sequence, head, keys or values, entry), four threads a token. Codes of values are
+// turned round in shared memory.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_kv8_read(Kv8Call a, const int32_t * first_of, Kv8Rows kr, Kv8Rows vr) {
-    constexpr int Q = D / 4;
+    constexpr int Q = D / 4, PITCH = D + 4;
     const int b = blockIdx.z, head = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1;
     const Kv8Entry e = kv8_entry(a, b);
     const int first = first_of ? max(first_of[b], 0) : 0;
     const int64_t blk = (int64_t) first / BLK + blockIdx.x;
     const int t = threadIdx.x / 4, d0 = (threadIdx.x % 4) * Q;
-    const int64_t i = blk * BLK + t - first;  // the token's place in the output
-    if (i < 0 || i >= a.b.max_new) return;
-    const Kv8Rows & r = is_v ? vr : kr;
-    T * out = (T *) (r.p + ((int64_t) b * r.entry + i * r.row + (int64_t) head * r.head) * 2) + d0;
+    __shared__ __align__(16) int8_t tile[BLK * PITCH];
     T x[Q];
 #pragma unroll
     for (int k = 0; k < Q; ++k) x[k] = (T) 0.0f;
-    if (e.seq >= 0 && blk * BLK + t < e.start) {
+    const bool held = blk * BLK + t < e.start;
+    if (e.seq >= 0 && blk * BLK < e.start) {
         if (blk == e.start / BLK) {
             const T * tail = (const T *) (is_v ? a.c.v_tail : a.c.k_tail) + ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
-            if (is_v) {
+            if (held && is_v) {
 #pragma unroll
                 for (int k = 0; k < Q; ++k) x[k] = tail[(d0 + k) * BLK + t];
-            } else {
+            } else if (held) {
                 load_row<T, Q>(tail + t * D + d0, true, x);
             }
         } else {
@@ -181,12 +180,30 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Call a, const int32_t * fir
             if (page >= 0) {
                 const float scale = (is_v ? a.c.v_scale : a.c.k_scale)[page * a.c.n_heads + head];
                 const int8_t * codes = (is_v ? a.c.v : a.c.k) + (page * a.c.n_heads + head) * BLK * D;
+                alignas(16) int8_t y[Q];
+                if (is_v) {
+                    for (int i = threadIdx.x; i < D * 4; i += 256) {
+                        alignas(16) int8_t z[16];
+                        *(u32x4 *) z = *(const u32x4 *) (codes + i * 16);
 #pragma unroll
-                for (int k = 0; k < Q; ++k) x[k] = (T) ((float) codes[is_v ? (d0 + k) * BLK + t : t * D + d0 + k] * scale);
+                        for (int k = 0; k < 16; ++k) tile[(i % 4 * 16 + k) * PITCH + i / 4] = z[k];
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int k = 0; k < Q / 4; ++k) *(uint32_t *) &y[k * 4] = *(const uint32_t *) &tile[t * PITCH + d0 + k * 4];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < Q / 16; ++k) *(u32x4 *) &y[k * 16] = *(const u32x4 *) (codes + t * D + d0 + k * 16);
+                }
+#pragma unroll
+                for (int k = 0; k < Q; ++k) x[k] = (T) ((float) y[k] * scale);
             }
         }
     }
-    store_row<T, Q>(out, r.vec, x);
+    const int64_t i = blk * BLK + t - first;  // the token's place in the output
+    if (i < 0 || i >= a.b.max_new) return;
+    const Kv8Rows & r = is_v ? vr : kr;
+    store_row<T, Q>((T *) (r.p + ((int64_t) b * r.entry + i * r.row + (int64_t) head * r.head) * 2) + d0, r.vec, x);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -198,15 +215,16 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Call a, const int32_t * fir
 // maximum m, sum l and accumulator of its own; the waves are joined in a fixed order at the end.
 //
 // Both products run on the codes themselves (16x16x64 i8 -> i32, exact): no code is ever converted. What
-// meets them is fixed point in two signed digits of 7 bits, value = unit * (128 * hi + lo):
-//   queries         unit = max|q| of the row / 16255: off by at most max|q| * 2^-15
-//   probabilities   exp2(s - block's maximum) in (0, 1], unit 1 / 16256: off by at most 2^-15 of the block's largest
+// meets them is fixed point in two signed bytes, value = unit * (256 * hi + lo), hi in +-127, lo in -128 .. 127:
+//   queries         unit = max|q| of the row / 32639: off by at most max|q| * 2^-15.99
+//   probabilities   exp2(s - block's maximum) in (0, 1], unit 1 / 32639: off by at most 2^-15.99 of the block's largest
+// The sums fit 32 bits: 128 * 127 * (256 * 127 + 128) < 2^30, so even the difference of two scores does.
 // The scale of a block multiplies the finished integer sums, in f32.
 //
 // Lanes: c = lane & 15 is the row (a column of S^T = K Q^T and of O^T = V^T P^T), g = lane >> 4. Key tile t
 // feeds key 16 (m >> 2) + 4 t + (m & 3) as row m, so lane (c, g) ends up with the scores of keys 16 g .. 16 g + 15
 // in order: exactly the 16 bytes of P^T that the second product wants of it. Nothing crosses lanes but the maximum.
-constexpr float QUNIT = 16255.0f, PUNIT = 16256.0f;
+constexpr float UNIT = 32639.0f;  // 256 * 127 + 127
 constexpr float LOG2E = 1.44269504088896340736f;
 
 __device__ __forceinline__ float max_over_g(float x) {
@@ -223,17 +241,14 @@ __device__ __forceinline__ float sum_over_g(float x) {
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-// the two digits of 16 values in [0, 16256], a byte each
-__device__ __forceinline__ void digits(const float (&p)[4][4], i32x4 & hi, i32x4 & lo) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        uint32_t x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = (uint32_t) fmaf(p[t][i], PUNIT, 0.5f);
-        const uint32_t a = x[0] | x[1] << 16, b = x[2] | x[3] << 16;
-        hi[t] = __builtin_amdgcn_perm(b >> 7, a >> 7, 0x06040200);
-        lo[t] = __builtin_amdgcn_perm(b, a, 0x06040200) & 0x7f7f7f7f;
-    }
+// The two bytes of four values in [-1, 1]. A float of 1.5 * 2^23 + z has the integer z in its low bits, so one fma rounds
+// to the unit; with z = value + 128, byte 1 of z is hi and byte 0 of it is lo + 128.
+__device__ __forceinline__ void digits(float x0, float x1, float x2, float x3, float unit, int & hi, int & lo) {
+    constexpr float MAGIC = 12582912.0f + 128.0f;
+    const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(fmaf(x1, unit, MAGIC)), __float_as_uint(fmaf(x0, unit, MAGIC)), 0x05040100);
+    const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(fmaf(x3, unit, MAGIC)), __float_as_uint(fmaf(x2, unit, MAGIC)), 0x05040100);
+    hi = __builtin_amdgcn_perm(b, a, 0x07050301);
+    lo = __builtin_amdgcn_perm(b, a, 0x06040200) ^ 0x80808080;
 }
 
 // a wave's state for its 16 rows
@@ -249,8 +264,8 @@ template <int D> struct Acc {
     // what a block brings has its own maximum mb (-inf: nothing of it is seen): the factor of its sums
     __device__ __forceinline__ float merge(float mb, float & alpha) {
         const float top = fmaxf(m, mb);
-        alpha = m == -INFINITY ? 0.0f : exp2f(m - top);
-        const float f = mb == -INFINITY ? 0.0f : exp2f(mb - top);
+        alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        const float f = mb == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mb - top);
         m = top;
         l *= alpha;
         return f;
@@ -269,6 +284,15 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
     typedef T vec8 __attribute__((ext_vector_type(8)));
     constexpr bool BF = !std::is_same<T, _Float16>::value;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    // values, dimension-major: lane (c, g) reads keys 16 g .. 16 g + 15 of dimension 16 dt + c
+    // (asked for before the scores where the registers allow it)
+    auto values = [&](int dt, int k) { return *(const vec8 *) (vt + (dt * 16 + c) * BLK + 16 * g + 8 * k); };
+    vec8 vx[D == 64 ? 4 : 1][2];
+    if (D == 64)
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) vx[D == 64 ? dt : 0][k] = values(dt, k);
     float s[4][4];
     {
         vec8 q[D / 32];
@@ -311,21 +335,21 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float p = exp2f(s[t][i] - base);
-            ls += p;
+            const float p = __builtin_amdgcn_exp2f(s[t][i] - base);
             const int k = t >> 1, e = 4 * (t & 1) + i;
             ph[k][e] = (T) (BF ? p : p * 16384.0f);
             if (BF) pl[k][e] = (T) (p - to_f32(ph[k][e]));
+            ls += BF ? p : to_f32(ph[k][e]);  // what is summed is what multiplies the values
         }
+    if (!BF) ls *= 1.0f / 16384.0f;
     uint32_t bad = 0;  // of the lane's 16 keys
     const float fo = BF ? f : f * (1.0f / 16384.0f);
-    // values, dimension-major: lane (c, g) reads keys 16 g .. 16 g + 15 of dimension 16 dt + c
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
         floatx4 x = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            vec8 v = *(const vec8 *) (vt + (dt * 16 + c) * BLK + 16 * g + 8 * k);
+            vec8 v = D == 64 ? vx[D == 64 ? dt : 0][k] : values(dt, k);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const bool mine = 16 * g + 8 * k + i < have, fine = finite(to_f32(v[i]));
@@ -346,90 +370,108 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
     acc.l += f * ls;
 }
 
-template <typename T, int D, typename O, int W>
-__global__ __launch_bounds__(W * 64) void k_kv8_attend_rows(Kv8Call a, Kv8Attend p) {
+// ONCE: no other tile reads these codes, they need not stay in the caches (cross attention of 32 clips 29.3 -> 26.7 us;
+// with more tiles of the same keys 141 -> 171 us, so then it is off)
+template <bool ONCE> __device__ __forceinline__ i32x4 load_codes(const int8_t * p) {
+    return ONCE ? __builtin_nontemporal_load((const i32x4 *) p) : *(const i32x4 *) p;
+}
+
+template <typename T, int D, typename O, int W, bool ONCE>
+__global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8Call a, Kv8Attend p) {
     constexpr int DT = D / 16, KC = D / 64;
     const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, head = blockIdx.y, b = blockIdx.z;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const Kv8Entry e = kv8_entry(a, b);
+    const int64_t page0 = kv8_page(a.c, e.seq, split * p.per + w);  // asked for together with the lengths
     const int rows = e.n * p.group - tile * 16;  // of this tile, and of those behind it
     if (rows <= 0) return;
     const int cap = a.c.max_blocks * BLK;
     const int stored = e.seq < 0 ? 0 : p.causal ? min(e.start + e.n, cap) : e.start;
     const int full = stored / BLK;
-    // what this lane's row sees, and what the tile sees at most
+    // what this lane's row sees, and what the tile sees at least and at most
     const int r = tile * 16 + c, qi = r / p.group;
     const int see = p.causal ? min(stored, e.start + qi + 1) : stored;
     const int last = min(tile * 16 + 15, e.n * p.group - 1) / p.group;
     const int most = p.causal ? min(stored, e.start + last + 1) : stored;
-    const int first = p.causal ? min(stored, e.start + tile * 16 / p.group + 1) : stored;  // the least a row of it sees
-    const int blocks = (most + BLK - 1) / BLK, per = (blocks + p.splits - 1) / p.splits;
-    const int lo = split * per, hi = min(blocks, lo + per);
+    const int least = p.causal ? min(stored, e.start + tile * 16 / p.group + 1) : stored;
+    const int blocks = (most + BLK - 1) / BLK, lo = split * p.per;
+    const int hi = split == p.splits - 1 ? blocks : min(blocks, lo + p.per);
+    if (split > 0 && lo >= hi) return;  // (the join looks at as many splits as the tile has)
 
     const T * qrow = c < rows ? (const T *) row_at(a, p.q, e, b, qi, head * p.group + r % p.group, 2) : nullptr;
-    const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
+    T qx[KC][16];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+        if (qrow) load_row<T, 16>(qrow + k * 64 + g * 16, p.q.vec, qx[k]);
+        else
+#pragma unroll
+            for (int i = 0; i < 16; ++i) qx[k][i] = (T) 0.0f;
+    }
+
+    // A block's keys are asked for as soon as the scores of the one before are made, its values when that one's are
+    // added: a wave always has loads in flight, and the first block's cover the queries' conversion.
+    const int koff = (16 * (c >> 2) + (c & 3)) * D + g * 16, voff = c * BLK + g * 16;
+    i32x4 kx[4][KC], vx[DT];
+    int64_t at = 0;
+    bool held;  // false: the block's table entry leads nowhere. Block 0 of the pool is read for it, and nothing is seen of it
+    float ks = 0.0f, sv = 0.0f;
+    auto ask_keys = [&](int64_t page) {
+        held = page >= 0;
+        at = (held ? page : 0) * a.c.n_heads + head;
+        const int8_t * kc = a.c.k + at * BLK * D + koff;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int k = 0; k < KC; ++k) kx[t][k] = load_codes<ONCE>(kc + 4 * t * D + k * 64);
+    };
+    auto ask_values = [&]() {
+        const int8_t * vc = a.c.v + at * BLK * D + voff;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) vx[dt] = load_codes<ONCE>(vc + dt * 16 * BLK);
+        ks = a.c.k_scale[at];
+        sv = a.c.v_scale[at];
+    };
+    const int codes = min(hi, full);  // blocks held in codes
+    int blk = lo + w;
+    ask_keys(blk < codes ? page0 : -1);
+    ask_values();
+
     i32x4 qh[KC], ql[KC];
     float qunit;
     {
-        T x[KC][16];
         float top = 0.0f;
         bool ok = true;
 #pragma unroll
-        for (int k = 0; k < KC; ++k) {
-            if (qrow) load_row<T, 16>(qrow + k * 64 + g * 16, p.q.vec, x[k]);
-            else
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[k][i] = (T) 0.0f;
+        for (int k = 0; k < KC; ++k)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float y = fabsf(to_f32(x[k][i]));
+                const float y = fabsf(to_f32(qx[k][i]));
                 ok &= finite(y);
                 top = fmaxf(top, y);
             }
-        }
         top = max_over_g(ok ? top : INFINITY);
-        const float inv = finite(top) && top > 0.0f ? QUNIT / top : 0.0f;
-        // a row whose largest element is so small that QUNIT / top overflows counts as zeros
-        qunit = finite(top) ? (finite(inv) ? top / QUNIT : 0.0f) * fabsf(p.scale) * LOG2E : NAN;
+        float inv = finite(top) && top > 0.0f ? UNIT / top : 0.0f;
+        // a row whose largest element is so small that UNIT / top overflows counts as zeros
+        qunit = finite(top) ? (finite(inv) ? top / UNIT : 0.0f) * fabsf(p.scale) * LOG2E : NAN;
+        inv = finite(inv) ? p.scale < 0.0f ? -inv : inv : 0.0f;
+        // what is not finite goes in as zero: the row's unit is NaN then
+        auto q = [&](int k, int i) { return ok ? to_f32(qx[k][i]) : 0.0f; };
 #pragma unroll
         for (int k = 0; k < KC; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                uint32_t h = 0, l = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int y = finite(inv) ? (int) rintf(to_f32(x[k][4 * j + i]) * inv * sgn) : 0;
-                    const int yh = (y + 64) >> 7;
-                    h |= (uint32_t) (yh & 255) << 8 * i;
-                    l |= (uint32_t) ((y - 128 * yh) & 255) << 8 * i;
-                }
+                int h, l;
+                digits(q(k, 4 * j), q(k, 4 * j + 1), q(k, 4 * j + 2), q(k, 4 * j + 3), inv, h, l);
                 qh[k][j] = h;
                 ql[k][j] = l;
             }
     }
 
     Acc<D> acc;
-    for (int blk = lo + w; blk < hi; blk += W) {
-        if (blk == full) {
-            const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
-            attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qrow, p.q.vec, p.scale * LOG2E,
-                              stored - full * BLK, see - full * BLK, acc);
-            continue;
-        }
-        const int64_t page = kv8_page(a.c, e.seq, blk);
-        if (page < 0) continue;
-        const int64_t at = page * a.c.n_heads + head;
-        const int8_t * kc = a.c.k + at * BLK * D;
-        const int8_t * vc = a.c.v + at * BLK * D;
-        i32x4 kx[4][KC], vx[DT];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int k = 0; k < KC; ++k) kx[t][k] = *(const i32x4 *) (kc + (16 * (c >> 2) + 4 * t + (c & 3)) * D + k * 64 + g * 16);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) vx[dt] = *(const i32x4 *) (vc + (dt * 16 + c) * BLK + g * 16);
-        const float f = qunit * a.c.k_scale[at], sv = a.c.v_scale[at];
-
+    for (; blk < codes; blk += W) {
+        const float f = qunit * ks, svl = sv;
+        const int here = held ? see - blk * BLK : 0;
+        const bool all = held && least >= blk * BLK + BLK;  // every row of the tile sees the whole block
         int s[4][4], top = INT_MIN;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -440,19 +482,13 @@ __global__ __launch_bounds__(W * 64) void k_kv8_attend_rows(Kv8Call a, Kv8Attend
                 xl = __builtin_amdgcn_mfma_i32_16x16x64_i8(kx[t][k], ql[k], xl, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][i] = xh[i] * 128 + xl[i];
+            for (int i = 0; i < 4; ++i) s[t][i] = xh[i] * 256 + xl[i];
         }
-        const int here = see - blk * BLK;
-        if (first < blk * BLK + BLK) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[t][i] = 16 * g + 4 * t + i < here ? s[t][i] : INT_MIN;
-        }
+        ask_keys(blk + W < codes ? kv8_page(a.c, e.seq, blk + W) : -1);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = max(top, s[t][i]);
+            for (int i = 0; i < 4; ++i) top = max(top, all || 16 * g + 4 * t + i < here ? s[t][i] : INT_MIN);
         top = max_over_g(top);
         const bool none = here <= 0;  // this row sees nothing of the block
         const float mb = none ? -INFINITY : (float) top * f;
@@ -462,23 +498,45 @@ __global__ __launch_bounds__(W * 64) void k_kv8_attend_rows(Kv8Call a, Kv8Attend
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // the difference of the integers is exact
-                pr[t][i] = s[t][i] == INT_MIN ? 0.0f : __builtin_amdgcn_exp2f((float) (s[t][i] - top) * f);
-                ls += pr[t][i];
-            }
-        acc.l += none ? 0.0f : fb * ls;
+            for (int i = 0; i < 4; ++i) pr[t][i] = __builtin_amdgcn_exp2f((float) (s[t][i] - top) * f);  // the difference is exact
+        if (!all) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pr[t][i] = 16 * g + 4 * t + i < here ? pr[t][i] : 0.0f;
+        }
         i32x4 ph, pl;
-        digits(pr, ph, pl);
-        const float fo = none ? 0.0f : fb * sv * (1.0f / PUNIT);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            ls += (pr[t][0] + pr[t][1]) + (pr[t][2] + pr[t][3]);
+            int h, l;
+            digits(pr[t][0], pr[t][1], pr[t][2], pr[t][3], UNIT, h, l);
+            ph[t] = h;
+            pl[t] = l;
+        }
+        acc.l += none ? 0.0f : fb * ls;
+        const float fo = none ? 0.0f : fb * svl * (1.0f / UNIT);
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc.o[dt][i] *= alpha;
+        }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             const i32x4 z = {0, 0, 0, 0};
             const i32x4 xh = __builtin_amdgcn_mfma_i32_16x16x64_i8(vx[dt], ph, z, 0, 0, 0);
             const i32x4 xl = __builtin_amdgcn_mfma_i32_16x16x64_i8(vx[dt], pl, z, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc.o[dt][i] = fmaf((float) (xh[i] * 128 + xl[i]), fo, acc.o[dt][i] * alpha);
+            for (int i = 0; i < 4; ++i) acc.o[dt][i] = fmaf((float) (xh[i] * 256 + xl[i]), fo, acc.o[dt][i]);
         }
+        ask_values();
+    }
+
+    if (blk == full && blk < hi) {
+        const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
+        attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qrow, p.q.vec, p.scale * LOG2E, stored - full * BLK,
+                          see - full * BLK, acc);
     }
 
     // join the waves, in order
@@ -495,7 +553,7 @@ __global__ __launch_bounds__(W * 64) void k_kv8_attend_rows(Kv8Call a, Kv8Attend
     }
     __syncthreads();
     const int n = min(rows, 16);
-    float * ws = p.ws + ((((int64_t) b * a.c.n_heads + head) * (gridDim.x / p.splits) + tile) * p.splits + split) * 16 * (D + 2);
+    float * ws = p.ws + ((((int64_t) b * a.c.n_heads + head) * p.tiles + tile) * p.splits + split) * 16 * (D + 2);
     for (int i = threadIdx.x; i < n * D; i += W * 64) {
         const int row = i / D, d = i % D;
         float top = -INFINITY, sum = 0.0f, x = 0.0f;
@@ -503,7 +561,7 @@ __global__ __launch_bounds__(W * 64) void k_kv8_attend_rows(Kv8Call a, Kv8Attend
         for (int k = 0; k < W; ++k) top = fmaxf(top, ml[k][row][0]);
 #pragma unroll
         for (int k = 0; k < W; ++k) {
-            const float f = ml[k][row][0] == -INFINITY ? 0.0f : exp2f(ml[k][row][0] - top);
+            const float f = ml[k][row][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k][row][0] - top);
             // (a NaN maximum is in no fmaxf: its wave's l is NaN and is kept)
             sum += f * ml[k][row][1] + (ml[k][row][1] == ml[k][row][1] ? 0.0f : NAN);
             x += f * o[k][row][d];
@@ -518,25 +576,389 @@ __global__ __launch_bounds__(W * 64) void k_kv8_attend_rows(Kv8Call a, Kv8Attend
     }
 }
 
-// joins the splits of a tile, in order
-template <int D, typename O> __global__ __launch_bounds__(256) void k_kv8_attend_join(Kv8Call a, Kv8Attend p) {
-    const int tile = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
-    const Kv8Entry e = kv8_entry(a, b);
-    const int n = min(e.n * p.group - tile * 16, 16);
-    const float * ws = p.ws + (((int64_t) b * a.c.n_heads + head) * gridDim.x + tile) * p.splits * 16 * (D + 2);
-    for (int i = threadIdx.x; i < n * D; i += 256) {
-        const int row = i / D, d = i % D;
-        float top = -INFINITY, sum = 0.0f, x = 0.0f;
-        for (int k = 0; k < p.splits; ++k) top = fmaxf(top, ws[(k * 16 + row) * (D + 2)]);
-        for (int k = 0; k < p.splits; ++k) {
-            const float * y = ws + (k * 16 + row) * (D + 2);
-            const float f = y[0] == -INFINITY ? 0.0f : exp2f(y[0] - top);
-            sum += f * y[1] + (y[1] == y[1] ? 0.0f : NAN);
-            x += f * y[2 + d];
-        }
-        const int q = tile * 16 + row;
-        ((O *) row_at(a, p.out, e, b, q / p.group, head * p.group + q % p.group, sizeof(O)))[d] = (O) (sum == 0.0f ? 0.0f : x / sum);
+// ---------------------------------------------------------------------------------------------------
+// attend, many rows
+// ---------------------------------------------------------------------------------------------------
+// Four waves of 32 rows each go through the blocks of their entry and head together. With that many rows what counts
+// is the work a score costs, so here a block's codes become half-precision floats once (exactly: they are integers up
+// to 127) on their way to shared memory, and both products are 16x16x32 f16 with f32 sums: a score then costs a fused
+// multiply-add, an exponential, a sum and half a conversion.
+//
+// The lanes hold what they hold above: S^T = K Q^T with the keys of a tile permuted so that lane (c, g) gets the scores of
+// keys 16 g .. 16 g + 15, and chunk k of eight of them is what O^T = V^T P^T wants as its k-th operand.
+// Probabilities are p = exp2(s - m) times 2^6 sv / sigma, sv the block's scale of values, sigma a power of two above
+// all of them so far: the accumulator is in units of sigma 2^-6 and the block's scale costs nothing. A block whose sv is
+// less than sigma 2^-20 (it would come near the end of half precision) is summed apart and scaled in f32. m follows the
+// running maximum only when that has grown by more than 8, so p stays below 2^8 and the accumulator is rarely rescaled.
+constexpr int MW = 4;           // waves
+constexpr int MR = 2;           // row tiles of a wave
+constexpr int MROWS = MW * MR * 16;
+
+// sixteen codes as half-precision floats: 0x6400 | x is 1024 + x
+__device__ __forceinline__ void to_half(const i32x4 & c, half8 (&h)[2]) {
+    const half2v off = {(_Float16) 1152.0f, (_Float16) 1152.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = (uint32_t) c[i] ^ 0x80808080;
+        const half2v a = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464, x, 0x04010400)) - off;
+        const half2v b = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464, x, 0x04030402)) - off;
+        h[i / 2][4 * (i % 2)] = a[0];
+        h[i / 2][4 * (i % 2) + 1] = a[1];
+        h[i / 2][4 * (i % 2) + 2] = b[0];
+        h[i / 2][4 * (i % 2) + 3] = b[1];
     }
+}
+
+template <int D> struct Stage {
+    // rows of keys and of value dimensions, 16-byte chunks xor-ed with a number of the row: eight lanes that read the
+    // same chunk of eight rows meet different banks
+    half8 k[BLK * D / 8], v[D * BLK / 8];
+    static __device__ __forceinline__ int at_k(int key, int chunk) { return key * (D / 8) + (chunk ^ ((key & 3) | (key >> 2 & 4))); }
+    static __device__ __forceinline__ int at_v(int d, int chunk) { return d * (BLK / 8) + (chunk ^ (d & 7)); }
+};
+
+template <typename T, int D, typename O>
+__global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8Attend p, int tiles) {
+    constexpr int DT = D / 16, KC = D / 32, NC = D / 64;  // NC: 16-byte pieces of codes of a thread
+    constexpr bool BF = !std::is_same<T, _Float16>::value;
+    __shared__ __align__(16) Stage<D> st[2];
+    __shared__ float red[2][MW];
+    __shared__ unsigned long long odd_keys;
+    // the tiles of one entry and head run on one of the eight dies (workgroups go round them): their keys stay in its
+    // cache; tiles that see the most keys go first
+    const int id = blockIdx.x, group = (id & 7) + 8 * (id / (8 * tiles * p.splits)), rest = id / 8 % (tiles * p.splits);
+    if (group >= a.c.n_heads * a.b.n) return;
+    const int head = group % a.c.n_heads, b = group / a.c.n_heads;
+    const int split = rest % p.splits, tile = tiles - 1 - rest / p.splits;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const Kv8Entry e = kv8_entry(a, b);
+    const int nrows = e.n * p.group;
+    if (tile * MROWS >= nrows) return;
+    const int cap = a.c.max_blocks * BLK;
+    const int stored = e.seq < 0 ? 0 : p.causal ? min(e.start + e.n, cap) : e.start;
+    const int full = stored / BLK;
+    auto sees = [&](int row) { return p.causal ? min(stored, e.start + min(row, nrows - 1) / p.group + 1) : stored; };
+    const int row0 = tile * MROWS + w * MR * 16;
+    const int most = sees(tile * MROWS + MROWS - 1);          // of the workgroup
+    const int mine = row0 < nrows ? sees(row0 + MR * 16 - 1) : 0, least = sees(row0);  // of the wave
+    const int blocks = (most + BLK - 1) / BLK, lo = split * p.per;
+    const int hi = split == p.splits - 1 ? blocks : min(blocks, lo + p.per);
+    if (split > 0 && lo >= hi) return;
+
+    // queries
+    half8 q[MR][KC];
+    float unit[MR];
+    int see[MR];
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+        const int row = row0 + r * 16 + c;
+        see[r] = row < nrows ? sees(row) : 0;
+        const T * qr = row < nrows ? (const T *) row_at(a, p.q, e, b, row / p.group, head * p.group + row % p.group, 2) : nullptr;
+        T x[KC][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            if (qr) load_row<T, 8>(qr + k * 32 + g * 8, p.q.vec, x[k]);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[k][i] = (T) 0.0f;
+            if (BF)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, finite(to_f32(x[k][i])) ? fabsf(to_f32(x[k][i])) : 0.0f);
+        }
+        // bf16 rows are brought to [1, 2) by a power of two, exact but for what is 2^-14 of the largest or less
+        int ex = 0;
+        if (BF) {
+            top = max_over_g(top);
+            ex = top > 0.0f ? ilogbf(top) : 0;
+        }
+        unit[r] = ldexpf(fabsf(p.scale) * LOG2E, ex);
+        const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[r][k][i] = (_Float16) (BF ? ldexpf(to_f32(x[k][i]), -ex) * sgn : to_f32(x[k][i]) * sgn);
+    }
+
+    // staging: 16 codes of keys and of values a thread and piece
+    i32x4 nk[NC], nv[NC];
+    int64_t at = 0;
+    bool held = false;
+    auto ask = [&](int blk) {
+        const int64_t page = blk < min(hi, full) ? kv8_page(a.c, e.seq, blk) : -1;
+        held = page >= 0;
+        at = (held ? page : 0) * a.c.n_heads + head;  // (block 0 of the pool is read for a block that is not there)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            nk[i] = ((const i32x4 *) (a.c.k + at * BLK * D))[threadIdx.x + i * 256];
+            nv[i] = ((const i32x4 *) (a.c.v + at * BLK * D))[threadIdx.x + i * 256];
+        }
+    };
+    auto put = [&](Stage<D> & s) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int n = threadIdx.x + i * 256;
+            half8 h[2];
+            to_half(nk[i], h);
+            s.k[Stage<D>::at_k(n / (D / 16), n % (D / 16) * 2)] = h[0];
+            s.k[Stage<D>::at_k(n / (D / 16), n % (D / 16) * 2 + 1)] = h[1];
+            to_half(nv[i], h);
+            s.v[Stage<D>::at_v(n / 4, n % 4 * 2)] = h[0];
+            s.v[Stage<D>::at_v(n / 4, n % 4 * 2 + 1)] = h[1];
+        }
+    };
+
+    const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    float m[MR], l[MR];  // the same in all four lanes of a row
+    floatx4 o[MR][DT];
+    int sig = INT_MIN;  // sigma = 2^sig
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] = floatx4{0, 0, 0, 0};
+    }
+
+    // a staged block: ks, sv its scales, there: its tokens that are held, bad: of those, the ones that are not finite (tail)
+    auto work = [&](const Stage<D> & s, int blk, float ks, float sv, bool there, uint32_t bad) {
+        const int base = blk * BLK;
+        const bool all = there && least >= base + BLK && row0 + MR * 16 <= nrows;
+        const int up = sv > 0.0f && finite(sv) ? ilogbf(sv) + 1 : INT_MIN;
+        const bool apart = up != INT_MIN && sig != INT_MIN && up < sig - 20;
+        const int old = sig;
+        if (up > sig) sig = up;
+        // what a probability is multiplied by, as a power of two, and what its sum is divided by
+        const float mul = apart || up == INT_MIN ? 64.0f : ldexpf(sv, 6 - sig);
+        const float lg = sv == sv ? __builtin_amdgcn_logf(mul) : NAN, inv = sv == sv ? 1.0f / mul : NAN;
+        floatx4 x[MR][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int key = 16 * (c >> 2) + 4 * t + (c & 3);
+#pragma unroll
+            for (int r = 0; r < MR; ++r) x[r][t] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                const half8 kk = s.k[Stage<D>::at_k(key, k * 4 + g)];
+#pragma unroll
+                for (int r = 0; r < MR; ++r) x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][k], x[r][t], 0, 0, 0);
+            }
+        }
+        half8 ph[MR][2];
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+            const int here = there ? see[r] - base : 0;
+            const float f = unit[r] * ks;
+            if (!all) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[r][t][i] = 16 * g + 4 * t + i < here ? x[r][t][i] : -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) top = fmaxf(fmaxf(fmaxf(x[r][t][0], x[r][t][1]), fmaxf(x[r][t][2], x[r][t][3])), top);
+            top = max_over_g(top);
+            const float mb = top == -INFINITY ? -INFINITY : top * f;
+            const bool grown = mb > m[r] + 8.0f || (m[r] == -INFINITY && mb > m[r]);
+            if (__any(grown) || (sig != old && old != INT_MIN)) {
+                const float next = grown ? mb : m[r];
+                float alpha = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - next);
+                m[r] = next;
+                l[r] *= alpha;
+                if (old != INT_MIN) alpha = ldexpf(alpha, old - sig);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[r][d][i] *= alpha;
+            }
+            const float mm = (m[r] == -INFINITY ? 0.0f : m[r]) - lg;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float y = __builtin_amdgcn_exp2f(fmaf(x[r][t][i], f, -mm));
+                    if (!all) y = 16 * g + 4 * t + i < here ? y : 0.0f;
+                    ph[r][t >> 1][4 * (t & 1) + i] = (_Float16) y;
+                }
+            // what is summed is what multiplies the values, by a product with ones
+            floatx4 sum = {0, 0, 0, 0};
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[r][0], sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[r][1], sum, 0, 0, 0);
+            if (here > 0) l[r] = fmaf(sum[0], inv, l[r]);
+            if (__any(bad != 0)) {
+                const int hit = max_over_g((int) (bad & ((1u << min(max(here - 16 * g, 0), 16)) - 1)));
+                if (hit) l[r] = NAN;
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const half8 v0 = s.v[Stage<D>::at_v(d * 16 + c, 2 * g)], v1 = s.v[Stage<D>::at_v(d * 16 + c, 2 * g + 1)];
+#pragma unroll
+            for (int r = 0; r < MR; ++r) {
+                if (!apart) {
+                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[r][0], o[r][d], 0, 0, 0);
+                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[r][1], o[r][d], 0, 0, 0);
+                } else {
+                    floatx4 y = {0, 0, 0, 0};
+                    y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[r][0], y, 0, 0, 0);
+                    y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[r][1], y, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[r][d][i] = fmaf(y[i], ldexpf(sv, -sig), o[r][d][i]);
+                }
+            }
+        }
+    };
+
+    const int codes = min(hi, full);
+    ask(lo);
+    if (lo < codes) put(st[0]);
+    __syncthreads();
+    for (int blk = lo; blk < codes; ++blk) {
+        const bool there = held;
+        const float ks = a.c.k_scale[at], sv = a.c.v_scale[at];
+        ask(blk + 1);
+        if (mine > blk * BLK) work(st[(blk - lo) & 1], blk, ks, sv, there, 0);
+        if (blk + 1 < codes) put(st[(blk + 1 - lo) & 1]);
+        __syncthreads();
+    }
+    if (full < hi && full >= lo) {
+        // the tail, from its 16-bit values; bf16 is brought into the range of f16 by a power of two, as queries are
+        const int have = stored - full * BLK;
+        const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
+        const T * kt = (const T *) a.c.k_tail + t;
+        const T * vt = (const T *) a.c.v_tail + t;
+        if (threadIdx.x == 0) odd_keys = 0;
+        __syncthreads();
+        float tk = 0.0f, tv = 0.0f;
+        unsigned long long bad = 0;
+        for (int n = threadIdx.x; n < BLK * D / 8; n += 256) {
+            T x[8];
+            load_row<T, 8>(kt + n * 8, true, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (n / (D / 8) < have && finite(to_f32(x[i]))) tk = fmaxf(tk, fabsf(to_f32(x[i])));
+            load_row<T, 8>(vt + n * 8, true, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = n % (BLK / 8) * 8 + i;
+                const float y = fabsf(to_f32(x[i]));
+                if (key < have) {
+                    if (finite(y)) tv = fmaxf(tv, y);
+                    else bad |= 1ull << key;
+                }
+            }
+        }
+        if (bad) atomicOr(&odd_keys, bad);  // (bits: their order does not matter)
+        tk = wave_max(tk);
+        tv = wave_max(tv);
+        if (lane == 0) {
+            red[0][w] = tk;
+            red[1][w] = tv;
+        }
+        __syncthreads();
+        int ek = 0, ev = 0;
+        if (BF) {
+            tk = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+            tv = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+            ek = tk > 0.0f ? ilogbf(tk) : 0;
+            ev = tv > 0.0f ? ilogbf(tv) : 0;
+        }
+        Stage<D> & s = st[0];
+        for (int n = threadIdx.x; n < BLK * D / 8; n += 256) {
+            T x[8];
+            half8 h;
+            load_row<T, 8>(kt + n * 8, true, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = n / (D / 8) < have ? to_f32(x[i]) : 0.0f;
+                h[i] = (_Float16) (BF ? ldexpf(y, -ek) : y);
+            }
+            s.k[Stage<D>::at_k(n / (D / 8), n % (D / 8))] = h;
+            load_row<T, 8>(vt + n * 8, true, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float y = to_f32(x[i]);
+                if (n % (BLK / 8) * 8 + i >= have || !finite(y)) y = 0.0f;
+                h[i] = (_Float16) (BF ? ldexpf(y, -ev) : y);
+            }
+            s.v[Stage<D>::at_v(n / (BLK / 8), n % (BLK / 8))] = h;
+        }
+        __syncthreads();
+        if (mine > full * BLK) work(s, full, ldexpf(1.0f, ek), ldexpf(1.0f, ev), true, (uint32_t) (odd_keys >> 16 * g) & 0xffff);
+    }
+
+    // lane (c, g) holds dimensions 16 d + 4 g .. + 3 of its rows
+    const float fin = sig == INT_MIN ? 0.0f : ldexpf(1.0f, sig - 6);
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+        const int row = row0 + r * 16 + c;
+        const float sum = l[r];
+        if (row >= nrows) continue;
+        if (p.splits > 1) {
+            const int64_t t16 = (int64_t) tiles * (MROWS / 16);
+            float * ws = p.ws + (((((int64_t) b * a.c.n_heads + head) * t16 + row / 16) * p.splits + split) * 16 + row % 16) * (D + 2);
+            if (g == 0) {
+                ws[0] = m[r];
+                ws[1] = sum;
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ws[2 + d * 16 + 4 * g + i] = o[r][d][i] * fin;
+        } else {
+            O * out = (O *) row_at(a, p.out, e, b, row / p.group, head * p.group + row % p.group, sizeof(O));
+            const float f = sum == 0.0f ? 0.0f : fin / sum;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[d * 16 + 4 * g + i] = (O) (sum == 0.0f ? 0.0f : o[r][d][i] * f);
+        }
+    }
+}
+
+// joins the splits of a row, in order: a workgroup a row, its waves take every fourth split and are joined at the end
+template <int D, typename O> __global__ __launch_bounds__(256) void k_kv8_attend_join(Kv8Call a, Kv8Attend p) {
+    constexpr int DL = D / 64;
+    const int r = blockIdx.x, tile = r / 16, row = r % 16, head = blockIdx.y, b = blockIdx.z;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const Kv8Entry e = kv8_entry(a, b);
+    if (r >= e.n * p.group) return;
+    const int stored = e.seq < 0 ? 0 : p.causal ? min(e.start + e.n, a.c.max_blocks * BLK) : e.start;
+    const int last = min((tile / p.join + 1) * p.join * 16 - 1, e.n * p.group - 1) / p.group;
+    const int most = p.causal ? min(stored, e.start + last + 1) : stored;
+    const int n = min(p.splits, max(1, ((most + BLK - 1) / BLK + p.per - 1) / p.per));
+    const float * ws = p.ws + ((((int64_t) b * a.c.n_heads + head) * p.tiles + tile) * p.splits * 16 + row) * (D + 2);
+    float m = -INFINITY, l = 0.0f, x[DL] = {};
+#pragma unroll 4
+    for (int k = w; k < n; k += 4) {
+        const float * y = ws + (int64_t) k * 16 * (D + 2);
+        const float mk = y[0], lk = y[1], top = fmaxf(m, mk);
+        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top), f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - top);
+        m = top;
+        l = l * alpha + (lk == lk ? f * lk : NAN);  // a split whose maximum is NaN has that l too
+#pragma unroll
+        for (int i = 0; i < DL; ++i) x[i] = x[i] * alpha + f * y[2 + i * 64 + lane];
+    }
+    __shared__ float ml[4][2], o[4][D];
+    if (lane == 0) {
+        ml[w][0] = m;
+        ml[w][1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < DL; ++i) o[w][i * 64 + lane] = x[i];
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    const int d = threadIdx.x;
+    const float top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0]));
+    float sum = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float f = ml[k][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k][0] - top);
+        sum += ml[k][1] == ml[k][1] ? f * ml[k][1] : NAN;
+        v += f * o[k][d];
+    }
+    ((O *) row_at(a, p.out, e, b, r / p.group, head * p.group + r % p.group, sizeof(O)))[d] = (O) (sum == 0.0f ? 0.0f : v / sum);
 }
 
 // blocks of a sequence that n consecutive tokens can touch
@@ -568,34 +990,51 @@ void kv8_read(hipStream_t s, const Kv8Call & call, const int32_t * first, const 
     });
 }
 
-// Splits: enough workgroups to fill the card, but no more than leaves a wave a block of its own
+// How a call is run. Up to 32 rows of an entry and head (a step, beams, grouped heads) go in tiles of 16, more in tiles of
+// 128. The keys are cut into parts of `per` blocks, a workgroup each. Entries may differ much in length, so parts are equal
+// in size and not in number: long entries have more of them.
 Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) {
-    const int64_t tiles = ((int64_t) call.b.max_new * group + 15) / 16;
-    const int64_t groups = tiles * call.c.n_heads * call.b.n;
-    const int64_t blocks = (max_len + BLK - 1) / BLK;
-    int64_t splits = 1;
-    if (groups < 512) splits = std::min((1024 + groups - 1) / groups, (blocks + 3) / 4);
-    if (blocks <= 32) splits = 1;
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, 256));
+    const int64_t rows = (int64_t) call.b.max_new * group;
+    const int64_t blocks = std::max<int64_t>(1, (max_len + BLK - 1) / BLK);
     Kv8Plan plan;
-    plan.splits = (int) splits;
-    plan.ws_bytes = splits > 1 ? (size_t) (groups * splits * 16 * (call.c.head_dim + 2)) * 4 : 0;
+    plan.many = rows > 32;
+    const int64_t tiles = plan.many ? (rows + MROWS - 1) / MROWS : (rows + 15) / 16;
+    const int64_t groups = tiles * call.c.n_heads * call.b.n;
+    int64_t per = blocks;
+    // few rows: 256 parts fill the card; parts of more than 32 blocks leave it unevenly loaded where lengths differ
+    if (!plan.many && blocks > 32) per = std::min<int64_t>(32, std::max<int64_t>(8, (groups * blocks + 255) / 256));
+    if (plan.many && groups < 256 && blocks > 16) per = std::max<int64_t>(8, (groups * blocks + 511) / 512);
+    plan.splits = (int) ((blocks + per - 1) / per);
+    plan.per = (int) ((blocks + plan.splits - 1) / plan.splits);
+    plan.tiles = (int) (plan.many ? tiles * (MROWS / 16) : tiles);
+    plan.ws_bytes = plan.splits > 1 ? (size_t) plan.tiles * call.c.n_heads * call.b.n * plan.splits * 16 * (call.c.head_dim + 2) * 4 : 0;
+    // few workgroups: eight waves rather than four share a tile's blocks
+    plan.wide = !plan.many && plan.splits == 1 && groups <= 256;
     return plan;
 }
 
-void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, int out_type) {
-    const int tiles = (int) (((int64_t) call.b.max_new * a.group + 15) / 16);
-    const dim3 grid(tiles * a.splits, call.c.n_heads, call.b.n), join(tiles, call.c.n_heads, call.b.n);
+void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, const Kv8Plan & plan, int out_type) {
+    const int rows = call.b.max_new * a.group;
+    const dim3 grid(plan.tiles * plan.splits, call.c.n_heads, call.b.n), join(rows, call.c.n_heads, call.b.n);
     with_type(call.c, [&](auto t, auto d) {
         using T = decltype(t);
         constexpr int D = decltype(d)::value;
-        if (out_type == OWK_KV8_F32) {
-            OWK_LAUNCH((k_kv8_attend_rows<T, D, float, 4>), grid, dim3(256), 0, s, call, a);
-            if (a.splits > 1) OWK_LAUNCH((k_kv8_attend_join<D, float>), join, dim3(256), 0, s, call, a);
-        } else {
-            OWK_LAUNCH((k_kv8_attend_rows<T, D, T, 4>), grid, dim3(256), 0, s, call, a);
-            if (a.splits > 1) OWK_LAUNCH((k_kv8_attend_join<D, T>), join, dim3(256), 0, s, call, a);
-        }
+        auto run = [&](auto o) {
+            using O = decltype(o);
+            if (plan.many) {
+                const int tiles = plan.tiles / (MROWS / 16), groups = (call.c.n_heads * call.b.n + 7) / 8 * 8;
+                OWK_LAUNCH((k_kv8_attend_tiles<T, D, O>), dim3(groups * tiles * plan.splits), dim3(MW * 64), 0, s, call, a, tiles);
+            } else if (plan.wide) {
+                if (plan.tiles == 1) OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 8, true>), grid, dim3(512), 0, s, call, a);
+                else OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 8, false>), grid, dim3(512), 0, s, call, a);
+            } else {
+                if (plan.tiles == 1) OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 4, true>), grid, dim3(256), 0, s, call, a);
+                else OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 4, false>), grid, dim3(256), 0, s, call, a);
+            }
+            if (plan.splits > 1) OWK_LAUNCH((k_kv8_attend_join<D, O>), join, dim3(256), 0, s, call, a);
+        };
+        if (out_type == OWK_KV8_F32) run(0.0f);
+        else run(t);
     });
 }
 

@@ -165,10 +165,13 @@ int owk_kv8_attend(const owk_kv8_cache * cache, const owk_kv8_batch * batch, con
     a.group = params->n_q_heads / cache->n_heads;
     a.causal = params->causal != 0;
     a.splits = plan.splits;
+    a.per = plan.per;
+    a.tiles = plan.tiles;
+    a.join = plan.many ? 8 : 1;
     a.scale = params->scale;
     a.ws = (float *) workspace;
     return on_device(cache->device,
-                     [&] { kv8_attend((hipStream_t) stream, Kv8Call{*cache, *batch}, a, params->out_type); });
+                     [&] { kv8_attend((hipStream_t) stream, Kv8Call{*cache, *batch}, a, plan, params->out_type); });
 }
 
 int owk_kv8_read(const owk_kv8_cache * cache, int n, int max_tokens, const int32_t * lens, const int32_t * seq,

@@ -61,20 +61,24 @@ struct Kv8Attend {
     Kv8Rows q, out;
     int group = 1;      // query heads of a key/value head
     int causal = 0;
-    int splits = 1;     // parts the keys of an entry are cut into, a workgroup each
+    int splits = 1;     // parts of `per` blocks that the keys of an entry are cut into at most, a workgroup each
+    int per = 0;
+    int tiles = 1;      // of 16 rows of an entry and head
+    int join = 1;       // of them in a workgroup
     float scale = 1.0f;
     float * ws = nullptr;
 };
 
 // the split and workspace of an attend call (host arithmetic on the call's sizes alone)
 struct Kv8Plan {
-    int splits;
+    int splits, per, tiles;
+    bool many, wide;
     size_t ws_bytes;
 };
 Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len);
 
 void kv8_append(hipStream_t s, const Kv8Call & call, const Kv8Rows & k, const Kv8Rows & v);
-void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, int out_type);
+void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, const Kv8Plan & plan, int out_type);
 void kv8_read(hipStream_t s, const Kv8Call & call, const int32_t * first, const Kv8Rows & k, const Kv8Rows & v);
 
 } // namespace owk

@@ -14,6 +14,7 @@ the cache's device. One layer of a model is one Cache; layers share lens. Bad ar
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch  # before the library: both use one HIP runtime
 
@@ -43,6 +44,10 @@ class AttendParams(C.Structure):
     _fields_ = [("n_q_heads", C.c_int), ("causal", C.c_int), ("out_type", C.c_int), ("max_len", C.c_int), ("scale", C.c_float)]
 
 
+# the same three structures as bytes: packing is several times quicker than filling a ctypes.Structure, and a call of one
+# token is as long on the host as on the GPU
+_BATCH, _ROWS, _PARAMS = struct.Struct("iiqPPPP").pack, struct.Struct("Pqqq").pack, struct.Struct("iiiif").pack
+
 _lib = None
 
 
@@ -50,13 +55,12 @@ def load():
     global _lib
     if _lib is None:
         L = owk.load()
-        cp, bp, rp, ap, vp = (C.POINTER(t) for t in (CacheDesc, Batch, Rows, AttendParams, C.c_char))
         vp = C.c_void_p
-        L.owk_kv8_append.argtypes = [cp, bp, rp, rp, vp]
-        L.owk_kv8_attend.argtypes = [cp, bp, ap, rp, rp, vp, C.c_size_t, vp]
-        L.owk_kv8_attend_workspace.argtypes = [cp, bp, ap]
+        L.owk_kv8_append.argtypes = [vp, vp, vp, vp, vp]
+        L.owk_kv8_attend.argtypes = [vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+        L.owk_kv8_attend_workspace.argtypes = [vp, vp, vp]
         L.owk_kv8_attend_workspace.restype = C.c_size_t
-        L.owk_kv8_read.argtypes = [cp, C.c_int, C.c_int, vp, vp, vp, rp, rp, vp]
+        L.owk_kv8_read.argtypes = [vp, C.c_int, C.c_int, vp, vp, vp, vp, vp, vp]
         L.owk_kv8_error.restype = C.c_char_p
         _lib = L
     return _lib
@@ -116,90 +120,104 @@ class Cache:
         self.desc = CacheDesc(dev.index, _TYPES[dtype], dim, heads, seqs, pool, blocks, k.data_ptr(), v.data_ptr(),
                               k_scale.data_ptr(), v_scale.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(),
                               table.data_ptr() if table is not None else None)
-        self._ref = C.byref(self.desc)
+        self._at = C.addressof(self.desc)
+        self._dev = dev.index
         self._L = load()
+        self._ws = {}
 
     def _index(self, name, x, n):
         if x is None:
-            return None
-        if x.dtype != torch.int32 or x.device != self.device or x.dim() != 1 or x.shape[0] != n or not x.is_contiguous():
+            return 0
+        if x.dtype is not torch.int32 or x.get_device() != self._dev or x.shape != (n,) or not x.is_contiguous():
             raise ValueError(f"{name} is {x.dtype} {tuple(x.shape)} on {x.device}, wanted contiguous int32 ({n},) on {self.device}")
         return x.data_ptr()
 
-    def _batch(self, x, lens, seq, off, count, max_new):
-        n = lens.shape[0]
-        if off is None:
-            if x.dim() != 4 or x.shape[0] != n:
-                raise ValueError(f"a padded tensor of {n} entries is [{n}, rows, heads, {self.head_dim}], got {tuple(x.shape)}")
-            most = x.shape[1]
-            if max_new is not None and max_new > most:
-                raise ValueError(f"max_new {max_new} passes the tensor's {most} rows")
-            return Batch(n, most if max_new is None else max_new, 0, self._index("lens", lens, n),
-                         self._index("seq", self._seq(seq, n), n), None, self._index("count", count, n))
-        if x.dim() != 3 or count is not None:
-            raise ValueError(f"joined tensors are [rows, heads, {self.head_dim}] without count, got {tuple(x.shape)}")
-        rows = x.shape[0]
-        return Batch(n, rows if max_new is None else max_new, rows, self._index("lens", lens, n),
-                     self._index("seq", self._seq(seq, n), n), self._index("off", off, n + 1), None)
-
-    def _seq(self, seq, n):
+    def _batch(self, shape, lens, seq, off, count, max_new):
+        n = lens.shape[0] if lens.dim() else 0
         if seq is None and n > self.n_seqs:
             raise ValueError(f"{n} entries, and the cache has {self.n_seqs} sequences")
-        return seq
+        rows = 0
+        if off is None:
+            if len(shape) != 4 or shape[0] != n:
+                raise ValueError(f"a padded tensor of {n} entries is [{n}, rows, heads, {self.head_dim}], got {tuple(shape)}")
+            if max_new is None:
+                max_new = shape[1]
+            elif max_new > shape[1]:
+                raise ValueError(f"max_new {max_new} passes the tensor's {shape[1]} rows")
+        else:
+            if len(shape) != 3 or count is not None:
+                raise ValueError(f"joined tensors are [rows, heads, {self.head_dim}] without count, got {tuple(shape)}")
+            rows = shape[0]
+            if max_new is None:
+                max_new = rows
+        return _BATCH(n, max_new, rows, self._index("lens", lens, n), self._index("seq", seq, n), self._index("off", off, n + 1),
+                      self._index("count", count, n)), n, max_new
 
-    def _rows(self, name, x, heads, dtype):
-        if x.dtype != dtype or x.device != self.device or x.shape[-1] != self.head_dim or (heads and x.shape[-2] != heads):
-            raise ValueError(f"{name} is {x.dtype} {tuple(x.shape)} on {x.device}, wanted {dtype} [.., {heads or 'heads'}, "
-                             f"{self.head_dim}] on {self.device}")
+    def _rows(self, name, x, shape, heads, dtype):
         s = x.stride()
+        if x.dtype is not dtype or x.get_device() != self._dev or shape[-1] != self.head_dim or shape[-2] != heads:
+            raise ValueError(f"{name} is {x.dtype} {tuple(shape)} on {x.device}, wanted {dtype} [.., {heads}, {self.head_dim}] "
+                             f"on {self.device}")
         if s[-1] != 1:
             raise ValueError(f"the innermost dimension of {name} is not contiguous")
-        return Rows(x.data_ptr(), s[0] if x.dim() == 4 else 0, s[-3], s[-2])
+        return _ROWS(x.data_ptr(), s[0] if len(s) == 4 else 0, s[-3], s[-2])
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self._dev)
 
     def append(self, k, v, lens, seq=None, off=None, count=None, max_new=None):
         """Store the entries' tokens behind the lens[b] that their sequences hold (or from an earlier multiple of 64 on)."""
-        b = self._batch(k, lens, seq, off, count, max_new)
-        if k.shape != v.shape:
-            raise ValueError(f"k is {tuple(k.shape)} and v is {tuple(v.shape)}")
-        kr, vr = self._rows("k", k, self.n_heads, self.dtype), self._rows("v", v, self.n_heads, self.dtype)
+        shape = k.shape
+        b, _, _ = self._batch(shape, lens, seq, off, count, max_new)
+        if shape != v.shape:
+            raise ValueError(f"k is {tuple(shape)} and v is {tuple(v.shape)}")
+        kr, vr = self._rows("k", k, shape, self.n_heads, self.dtype), self._rows("v", v, shape, self.n_heads, self.dtype)
         if k.numel():
-            _check(self._L.owk_kv8_append(self._ref, b, kr, vr, self._stream()))
+            _check(self._L.owk_kv8_append(self._at, b, kr, vr, self._stream()))
 
     def attend(self, q, lens, seq=None, off=None, count=None, max_new=None, max_len=0, scale=None, causal=False, out=None):
         """softmax(scale * q . k) . v over what the sequences hold: tokens [0, lens[b]), or with causal, for row i,
         [0, lens[b] + i] (its own tokens appended before). scale None: 1 / sqrt(head_dim). `max_len`: no sequence holds
         more (a hint for splitting the work). `out`: a tensor like q, or float32; rows that are no entry's stay as they are."""
-        b = self._batch(q, lens, seq, off, count, max_new)
-        heads = q.shape[-2]
-        qr = self._rows("q", q, 0, self.dtype)
+        shape = q.shape
+        b, n, max_new = self._batch(shape, lens, seq, off, count, max_new)
+        heads = shape[-2]
         if heads < 1 or heads % self.n_heads:
             raise ValueError(f"{heads} query heads are no multiple of {self.n_heads} key/value heads")
+        qr = self._rows("q", q, shape, heads, self.dtype)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape:
-            raise ValueError(f"out is {tuple(out.shape)} and q is {tuple(q.shape)}")
-        elif any(n > 1 and t == 0 for n, t in zip(out.shape, out.stride())):
+            out = torch.empty_like(q)
+            if 0 in out.stride():
+                out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        elif out.shape != shape:
+            raise ValueError(f"out is {tuple(out.shape)} and q is {tuple(shape)}")
+        elif any(i > 1 and t == 0 for i, t in zip(shape, out.stride())):
             raise ValueError("rows of out lie on each other")
-        p = AttendParams(heads, 1 if causal else 0, _TYPES.get(out.dtype, -1), max_len,
-                         self.head_dim ** -0.5 if scale is None else scale)
-        orow = self._rows("out", out, heads, torch.float32 if out.dtype == torch.float32 else self.dtype)
+        of = out.dtype
+        orow = self._rows("out", out, shape, heads, of if of is torch.float32 else self.dtype)
+        p = _PARAMS(heads, 1 if causal else 0, _TYPES[of], max_len, self.head_dim ** -0.5 if scale is None else scale)
         if q.numel():
-            n = self._L.owk_kv8_attend_workspace(self._ref, b, p)
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-            _check(self._L.owk_kv8_attend(self._ref, b, p, qr, orow, ws.data_ptr() if n else None, n, self._stream()))
+            need = self._ws.get((n, max_new, heads, max_len))
+            if need is None:  # a function of these sizes alone
+                if len(self._ws) >= 1024:
+                    self._ws.clear()
+                need = self._ws[(n, max_new, heads, max_len)] = self._L.owk_kv8_attend_workspace(self._at, b, p)
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            _check(self._L.owk_kv8_attend(self._at, b, p, qr, orow, ws.data_ptr() if need else None, need, self._stream()))
         return out
 
     def read(self, lens, max_tokens, seq=None, first=None):
         """Tokens first[b] (None: 0) .. + max_tokens of sequences that hold lens[b]: (k, v), each [entry, token, head,
         head_dim] in the cache's 16-bit type, zeros from lens[b] on."""
-        n = lens.shape[0]
-        k = torch.empty((n, max_tokens, self.n_heads, self.head_dim), dtype=self.dtype, device=self.device)
-        v = torch.empty_like(k)
-        i = [self._index("lens", lens, n), self._index("seq", self._seq(seq, n), n), self._index("first", first, n)]
-        if k.numel():
-            _check(self._L.owk_kv8_read(self._ref, n, max_tokens, *i, self._rows("k", k, 0, self.dtype),
-                                        self._rows("v", v, 0, self.dtype), self._stream()))
+        n = lens.shape[0] if lens.dim() else 0
+        if seq is None and n > self.n_seqs:
+            raise ValueError(f"{n} entries, and the cache has {self.n_seqs} sequences")
+        h, d = self.n_heads, self.head_dim
+        kv = torch.empty((2, n, max_tokens, h, d), dtype=self.dtype, device=self.device)
+        k, v = kv.unbind(0)
+        i = self._index("lens", lens, n), self._index("seq", seq, n), self._index("first", first, n)
+        if kv.numel():
+            at, one = kv.data_ptr(), max_tokens * h * d
+            _check(self._L.owk_kv8_read(self._at, n, max_tokens, *i, _ROWS(at, one, h * d, d),
+                                        _ROWS(at + 2 * n * one, one, h * d, d), self._stream()))
         return k, v

@@ -16,6 +16,8 @@ namespace {
 typedef __bf16 bf16_t;
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int BLK = kKv8Block;
@@ -227,13 +229,18 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Call a, const int32_t * fir
 constexpr float UNIT = 32639.0f;  // 256 * 127 + 127
 constexpr float LOG2E = 1.44269504088896340736f;
 
-__device__ __forceinline__ float max_over_g(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
-}
+// over the four lanes of a row: rows of 16 lanes, then halves of the wave, change places with each other
 __device__ __forceinline__ int max_over_g(int x) {
-    x = max(x, __shfl_xor(x, 16));
-    return max(x, __shfl_xor(x, 32));
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max((int) a[0], (int) a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max((int) b[0], (int) b[1]);
+}
+__device__ __forceinline__ float max_over_g(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float sum_over_g(float x) {
     x += __shfl_xor(x, 16);
@@ -586,10 +593,10 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
 //
 // The lanes hold what they hold above: S^T = K Q^T with the keys of a tile permuted so that lane (c, g) gets the scores of
 // keys 16 g .. 16 g + 15, and chunk k of eight of them is what O^T = V^T P^T wants as its k-th operand.
-// Probabilities are p = exp2(s - m) times 2^6 sv / sigma, sv the block's scale of values, sigma a power of two above
-// all of them so far: the accumulator is in units of sigma 2^-6 and the block's scale costs nothing. A block whose sv is
-// less than sigma 2^-20 (it would come near the end of half precision) is summed apart and scaled in f32. m follows the
-// running maximum only when that has grown by more than 8, so p stays below 2^8 and the accumulator is rarely rescaled.
+// Probabilities are p = exp2(s - m) times 2^6 sv / sigma, sv the block's scale of values, sigma a power of two above it: the
+// accumulator is in units of sigma 2^-6 and the block's scale costs nothing. sigma moves (and the accumulator with it, an
+// exact step) when a scale is larger, or 2^-20 smaller and so near the end of half precision. m follows the running
+// maximum only when that has grown by more than 8: p stays below 2^8, and the accumulator is rarely rescaled.
 constexpr int MW = 4;           // waves
 constexpr int MR = 2;           // row tiles of a wave
 constexpr int MROWS = MW * MR * 16;
@@ -680,14 +687,17 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
             for (int i = 0; i < 8; ++i) q[r][k][i] = (_Float16) (BF ? ldexpf(to_f32(x[k][i]), -ex) * sgn : to_f32(x[k][i]) * sgn);
     }
 
-    // staging: 16 codes of keys and of values a thread and piece
+    // staging of block blk into s: its codes are asked for a block ahead, 16 of keys and of values a thread and piece
+    const int codes = min(hi, full);  // blocks held in codes
     i32x4 nk[NC], nv[NC];
     int64_t at = 0;
-    bool held = false;
+    bool held = false;  // false: block 0 of the pool is read for a block that is not there, and nothing is seen of it
+    float ks = 0.0f, sv = 0.0f;
+    uint32_t bad = 0;   // tokens of the lane's 16 that are not finite (tail)
     auto ask = [&](int blk) {
-        const int64_t page = blk < min(hi, full) ? kv8_page(a.c, e.seq, blk) : -1;
+        const int64_t page = blk < codes ? kv8_page(a.c, e.seq, blk) : -1;
         held = page >= 0;
-        at = (held ? page : 0) * a.c.n_heads + head;  // (block 0 of the pool is read for a block that is not there)
+        at = (held ? page : 0) * a.c.n_heads + head;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             nk[i] = ((const i32x4 *) (a.c.k + at * BLK * D))[threadIdx.x + i * 256];
@@ -706,124 +716,11 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
             s.v[Stage<D>::at_v(n / 4, n % 4 * 2)] = h[0];
             s.v[Stage<D>::at_v(n / 4, n % 4 * 2 + 1)] = h[1];
         }
+        ks = a.c.k_scale[at];
+        sv = a.c.v_scale[at];
     };
-
-    const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-    float m[MR], l[MR];  // the same in all four lanes of a row
-    floatx4 o[MR][DT];
-    int sig = INT_MIN;  // sigma = 2^sig
-#pragma unroll
-    for (int r = 0; r < MR; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[r][d] = floatx4{0, 0, 0, 0};
-    }
-
-    // a staged block: ks, sv its scales, there: its tokens that are held, bad: of those, the ones that are not finite (tail)
-    auto work = [&](const Stage<D> & s, int blk, float ks, float sv, bool there, uint32_t bad) {
-        const int base = blk * BLK;
-        const bool all = there && least >= base + BLK && row0 + MR * 16 <= nrows;
-        const int up = sv > 0.0f && finite(sv) ? ilogbf(sv) + 1 : INT_MIN;
-        const bool apart = up != INT_MIN && sig != INT_MIN && up < sig - 20;
-        const int old = sig;
-        if (up > sig) sig = up;
-        // what a probability is multiplied by, as a power of two, and what its sum is divided by
-        const float mul = apart || up == INT_MIN ? 64.0f : ldexpf(sv, 6 - sig);
-        const float lg = sv == sv ? __builtin_amdgcn_logf(mul) : NAN, inv = sv == sv ? 1.0f / mul : NAN;
-        floatx4 x[MR][4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int key = 16 * (c >> 2) + 4 * t + (c & 3);
-#pragma unroll
-            for (int r = 0; r < MR; ++r) x[r][t] = floatx4{0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < KC; ++k) {
-                const half8 kk = s.k[Stage<D>::at_k(key, k * 4 + g)];
-#pragma unroll
-                for (int r = 0; r < MR; ++r) x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][k], x[r][t], 0, 0, 0);
-            }
-        }
-        half8 ph[MR][2];
-#pragma unroll
-        for (int r = 0; r < MR; ++r) {
-            const int here = there ? see[r] - base : 0;
-            const float f = unit[r] * ks;
-            if (!all) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[r][t][i] = 16 * g + 4 * t + i < here ? x[r][t][i] : -INFINITY;
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) top = fmaxf(fmaxf(fmaxf(x[r][t][0], x[r][t][1]), fmaxf(x[r][t][2], x[r][t][3])), top);
-            top = max_over_g(top);
-            const float mb = top == -INFINITY ? -INFINITY : top * f;
-            const bool grown = mb > m[r] + 8.0f || (m[r] == -INFINITY && mb > m[r]);
-            if (__any(grown) || (sig != old && old != INT_MIN)) {
-                const float next = grown ? mb : m[r];
-                float alpha = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - next);
-                m[r] = next;
-                l[r] *= alpha;
-                if (old != INT_MIN) alpha = ldexpf(alpha, old - sig);
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[r][d][i] *= alpha;
-            }
-            const float mm = (m[r] == -INFINITY ? 0.0f : m[r]) - lg;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float y = __builtin_amdgcn_exp2f(fmaf(x[r][t][i], f, -mm));
-                    if (!all) y = 16 * g + 4 * t + i < here ? y : 0.0f;
-                    ph[r][t >> 1][4 * (t & 1) + i] = (_Float16) y;
-                }
-            // what is summed is what multiplies the values, by a product with ones
-            floatx4 sum = {0, 0, 0, 0};
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[r][0], sum, 0, 0, 0);
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[r][1], sum, 0, 0, 0);
-            if (here > 0) l[r] = fmaf(sum[0], inv, l[r]);
-            if (__any(bad != 0)) {
-                const int hit = max_over_g((int) (bad & ((1u << min(max(here - 16 * g, 0), 16)) - 1)));
-                if (hit) l[r] = NAN;
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            const half8 v0 = s.v[Stage<D>::at_v(d * 16 + c, 2 * g)], v1 = s.v[Stage<D>::at_v(d * 16 + c, 2 * g + 1)];
-#pragma unroll
-            for (int r = 0; r < MR; ++r) {
-                if (!apart) {
-                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[r][0], o[r][d], 0, 0, 0);
-                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[r][1], o[r][d], 0, 0, 0);
-                } else {
-                    floatx4 y = {0, 0, 0, 0};
-                    y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[r][0], y, 0, 0, 0);
-                    y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[r][1], y, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[r][d][i] = fmaf(y[i], ldexpf(sv, -sig), o[r][d][i]);
-                }
-            }
-        }
-    };
-
-    const int codes = min(hi, full);
-    ask(lo);
-    if (lo < codes) put(st[0]);
-    __syncthreads();
-    for (int blk = lo; blk < codes; ++blk) {
-        const bool there = held;
-        const float ks = a.c.k_scale[at], sv = a.c.v_scale[at];
-        ask(blk + 1);
-        if (mine > blk * BLK) work(st[(blk - lo) & 1], blk, ks, sv, there, 0);
-        if (blk + 1 < codes) put(st[(blk + 1 - lo) & 1]);
-        __syncthreads();
-    }
-    if (full < hi && full >= lo) {
-        // the tail, from its 16-bit values; bf16 is brought into the range of f16 by a power of two, as queries are
+    // the tail, from its 16-bit values; bf16 is brought into the range of f16 by a power of two, as queries are
+    auto put_tail = [&](Stage<D> & s) {
         const int have = stored - full * BLK;
         const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
         const T * kt = (const T *) a.c.k_tail + t;
@@ -831,7 +728,7 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
         if (threadIdx.x == 0) odd_keys = 0;
         __syncthreads();
         float tk = 0.0f, tv = 0.0f;
-        unsigned long long bad = 0;
+        unsigned long long odd = 0;
         for (int n = threadIdx.x; n < BLK * D / 8; n += 256) {
             T x[8];
             load_row<T, 8>(kt + n * 8, true, x);
@@ -845,11 +742,11 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
                 const float y = fabsf(to_f32(x[i]));
                 if (key < have) {
                     if (finite(y)) tv = fmaxf(tv, y);
-                    else bad |= 1ull << key;
+                    else odd |= 1ull << key;
                 }
             }
         }
-        if (bad) atomicOr(&odd_keys, bad);  // (bits: their order does not matter)
+        if (odd) atomicOr(&odd_keys, odd);  // (bits: their order does not matter)
         tk = wave_max(tk);
         tv = wave_max(tv);
         if (lane == 0) {
@@ -864,7 +761,6 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
             ek = tk > 0.0f ? ilogbf(tk) : 0;
             ev = tv > 0.0f ? ilogbf(tv) : 0;
         }
-        Stage<D> & s = st[0];
         for (int n = threadIdx.x; n < BLK * D / 8; n += 256) {
             T x[8];
             half8 h;
@@ -884,8 +780,130 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
             }
             s.v[Stage<D>::at_v(n / (BLK / 8), n % (BLK / 8))] = h;
         }
+        held = true;
+        ks = ldexpf(1.0f, ek);
+        sv = ldexpf(1.0f, ev);
+        bad = (uint32_t) (odd_keys >> 16 * g) & 0xffff;
+    };
+
+    const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    float m[MR], l[MR];  // the same in all four lanes of a row
+    floatx4 o[MR][DT];
+    int sig = INT_MIN;  // sigma = 2^sig
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] = floatx4{0, 0, 0, 0};
+    }
+    const bool whole = row0 + MR * 16 <= nrows;  // all rows of the wave are there
+
+    ask(lo);
+    if (lo < codes) put(st[0]);
+    else if (lo < hi) put_tail(st[0]);
+    __syncthreads();
+    for (int blk = lo; blk < hi; ++blk) {
+        const Stage<D> & s = st[(blk - lo) & 1];
+        const int base = blk * BLK;
+        const bool there = held;
+        const float cks = ks, csv = sv;
+        const uint32_t cbad = bad;
+        ask(blk + 1);
+        if (mine > base) {
+            const bool part = !(there && whole && least >= base + BLK);  // some row does not see all of it
+            // sigma goes up with a larger scale, and down where a scale would come too near the end of half precision
+            const int up = csv > 0.0f && finite(csv) ? ilogbf(csv) + 1 : INT_MIN;
+            const int old = sig;
+            if (up != INT_MIN && (up > sig || up < sig - 20)) sig = old == INT_MIN ? up : max(up, old - 90);
+            const float moved = old == INT_MIN ? 1.0f : ldexpf(1.0f, old - sig);
+            // what a probability is multiplied by, and what its sum is divided by
+            const float mul = up == INT_MIN ? 64.0f : ldexpf(csv, 6 - sig);
+            const float lg = csv == csv ? __builtin_amdgcn_logf(mul) : NAN, inv = csv == csv ? 1.0f / mul : NAN;
+            floatx4 x[MR][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int key = 16 * (c >> 2) + 4 * t + (c & 3);
+#pragma unroll
+                for (int r = 0; r < MR; ++r) x[r][t] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < KC; ++k) {
+                    const half8 kk = s.k[Stage<D>::at_k(key, k * 4 + g)];
+#pragma unroll
+                    for (int r = 0; r < MR; ++r) x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][k], x[r][t], 0, 0, 0);
+                }
+            }
+            uint32_t ph[MR][8];  // pairs of probabilities: of keys 16 g + 2 j, + 1
+#pragma unroll
+            for (int r = 0; r < MR; ++r) {
+                const int here = part ? there ? see[r] - base : 0 : BLK;
+                const float f = unit[r] * cks;
+                float by = moved;  // what the accumulator is multiplied by
+                // the probabilities by the m there is; where they come out too large (or there is none yet), m is brought
+                // up to the maximum and they are made again
+#pragma clang loop unroll(disable)
+                for (int again = 0;; ++again) {
+                    const bool fresh = m[r] == -INFINITY;
+                    const float mm = (fresh ? 0.0f : m[r]) - lg;
+                    ushort2v big = {0, 0};  // as half-precision bits they are ordered like integers
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2v y = {__builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4], f, -mm)),
+                                           __builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4 + 1], f, -mm))};
+                        const ushort2v h = __builtin_bit_cast(ushort2v, __builtin_convertvector(y, half2v));
+                        big = __builtin_elementwise_max(big, h);
+                        ph[r][j] = __builtin_bit_cast(uint32_t, h);
+                    }
+                    const bool over = max(big[0], big[1]) > 0x7400 /* 2^14 */ || (fresh && here > 0);
+                    if (again || !__any(over)) break;
+                    float top = -INFINITY;
+                    int till = here - 16 * g;
+                    asm volatile("" : "+v"(till));  // (keeps the comparisons in here, out of every block's way)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, 4 * t + i < till ? x[r][t][i] : -INFINITY);
+                    top = max_over_g(top);
+                    const float mb = top == -INFINITY ? -INFINITY : top * f, next = fmaxf(m[r], mb);
+                    const float alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(m[r] - next);
+                    m[r] = next;
+                    l[r] *= alpha;
+                    by *= alpha;
+                }
+                if (part) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        ph[r][j] &= (16 * g + 2 * j < here ? 0xffffu : 0u) | (16 * g + 2 * j + 1 < here ? 0xffff0000u : 0u);
+                }
+                if (__any(by != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[r][d][i] *= by;
+                }
+                // what is summed is what multiplies the values, by a product with ones
+                floatx4 sum = {0, 0, 0, 0};
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, *(const half8 *) &ph[r][0], sum, 0, 0, 0);
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, *(const half8 *) &ph[r][4], sum, 0, 0, 0);
+                if (here > 0) l[r] = fmaf(sum[0], inv, l[r]);
+                if (__any(cbad != 0)) {
+                    const int hit = max_over_g((int) (cbad & ((1u << min(max(here - 16 * g, 0), 16)) - 1)));
+                    if (hit) l[r] = NAN;
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const half8 v0 = s.v[Stage<D>::at_v(d * 16 + c, 2 * g)], v1 = s.v[Stage<D>::at_v(d * 16 + c, 2 * g + 1)];
+#pragma unroll
+                for (int r = 0; r < MR; ++r) {
+                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, *(const half8 *) &ph[r][0], o[r][d], 0, 0, 0);
+                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, *(const half8 *) &ph[r][4], o[r][d], 0, 0, 0);
+                }
+            }
+        }
+        if (blk + 1 < codes) put(st[(blk + 1 - lo) & 1]);
+        else if (blk + 1 < hi) put_tail(st[(blk + 1 - lo) & 1]);
         __syncthreads();
-        if (mine > full * BLK) work(s, full, ldexpf(1.0f, ek), ldexpf(1.0f, ev), true, (uint32_t) (odd_keys >> 16 * g) & 0xffff);
     }
 
     // lane (c, g) holds dimensions 16 d + 4 g .. + 3 of its rows
@@ -910,9 +928,18 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
             O * out = (O *) row_at(a, p.out, e, b, row / p.group, head * p.group + row % p.group, sizeof(O));
             const float f = sum == 0.0f ? 0.0f : fin / sum;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d) {
+                typedef O vec4 __attribute__((ext_vector_type(4)));
+                vec4 y;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) out[d * 16 + 4 * g + i] = (O) (sum == 0.0f ? 0.0f : o[r][d][i] * f);
+                for (int i = 0; i < 4; ++i) y[i] = (O) (sum == 0.0f ? 0.0f : o[r][d][i] * f);
+                if (p.out.vec) {
+                    *(vec4 *) (out + d * 16 + 4 * g) = y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[d * 16 + 4 * g + i] = y[i];
+                }
+            }
         }
     }
 }

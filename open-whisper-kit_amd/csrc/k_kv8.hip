@@ -386,7 +386,17 @@ template <bool ONCE> __device__ __forceinline__ i32x4 load_codes(const int8_t * 
 template <typename T, int D, typename O, int W, bool ONCE>
 __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8Call a, Kv8Attend p) {
     constexpr int DT = D / 16, KC = D / 64;
-    const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, head = blockIdx.y, b = blockIdx.z;
+    // the tiles of one entry and head run on one of the eight dies (workgroups go round them): the keys they share stay in
+    // its cache
+    int head = blockIdx.y, b = blockIdx.z, split = 0, tile = 0;
+    if (gridDim.x > 1) {
+        const int id = blockIdx.x, group = (id & 7) + 8 * (id / (8 * p.tiles * p.splits)), rest = id / 8 % (p.tiles * p.splits);
+        if (group >= a.c.n_heads * a.b.n) return;
+        head = group % a.c.n_heads;
+        b = group / a.c.n_heads;
+        split = rest % p.splits;
+        tile = rest / p.splits;
+    }
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const Kv8Entry e = kv8_entry(a, b);
     const int64_t page0 = kv8_page(a.c, e.seq, split * p.per + w);  // asked for together with the lengths
@@ -597,9 +607,7 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
 // accumulator is in units of sigma 2^-6 and the block's scale costs nothing. sigma moves (and the accumulator with it, an
 // exact step) when a scale is larger, or 2^-20 smaller and so near the end of half precision. m follows the running
 // maximum only when that has grown by more than 8: p stays below 2^8, and the accumulator is rarely rescaled.
-constexpr int MW = 4;           // waves
-constexpr int MR = 2;           // row tiles of a wave
-constexpr int MROWS = MW * MR * 16;
+constexpr int MR = 2;  // row tiles of a wave
 
 // sixteen codes as half-precision floats: 0x6400 | x is 1024 + x
 __device__ __forceinline__ void to_half(const i32x4 & c, half8 (&h)[2]) {
@@ -616,17 +624,18 @@ __device__ __forceinline__ void to_half(const i32x4 & c, half8 (&h)[2]) {
     }
 }
 
+// a staged block: rows of keys and of value dimensions, their 16-byte chunks xor-ed with three bits of the row, so that eight
+// lanes that read the same chunk of eight rows meet different banks
 template <int D> struct Stage {
-    // rows of keys and of value dimensions, 16-byte chunks xor-ed with a number of the row: eight lanes that read the
-    // same chunk of eight rows meet different banks
     half8 k[BLK * D / 8], v[D * BLK / 8];
     static __device__ __forceinline__ int at_k(int key, int chunk) { return key * (D / 8) + (chunk ^ ((key & 3) | (key >> 2 & 4))); }
     static __device__ __forceinline__ int at_v(int d, int chunk) { return d * (BLK / 8) + (chunk ^ (d & 7)); }
 };
 
-template <typename T, int D, typename O>
-__global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8Attend p, int tiles) {
-    constexpr int DT = D / 16, KC = D / 32, NC = D / 64;  // NC: 16-byte pieces of codes of a thread
+template <typename T, int D, typename O, int MW>
+__global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(Kv8Call a, Kv8Attend p, int tiles) {
+    constexpr int MROWS = MW * MR * 16, NT = MW * 64;
+    constexpr int DT = D / 16, KC = D / 32, NC = BLK * D / 16 / NT;  // NC: 16-byte pieces of codes of a thread
     constexpr bool BF = !std::is_same<T, _Float16>::value;
     __shared__ __align__(16) Stage<D> st[2];
     __shared__ float red[2][MW];
@@ -690,34 +699,44 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
     // staging of block blk into s: its codes are asked for a block ahead, 16 of keys and of values a thread and piece
     const int codes = min(hi, full);  // blocks held in codes
     i32x4 nk[NC], nv[NC];
-    int64_t at = 0;
-    bool held = false;  // false: block 0 of the pool is read for a block that is not there, and nothing is seen of it
-    float ks = 0.0f, sv = 0.0f;
+    bool held = false, nheld;  // false: block 0 of the pool is read for a block that is not there, and nothing is seen of it
+    float ks = 0.0f, sv = 0.0f, nks, nsv;
+    int64_t page = lo < codes ? kv8_page(a.c, e.seq, lo) : -1;  // (a block's table entry, too, a block ahead of its codes)
     uint32_t bad = 0;   // tokens of the lane's 16 that are not finite (tail)
     auto ask = [&](int blk) {
-        const int64_t page = blk < codes ? kv8_page(a.c, e.seq, blk) : -1;
-        held = page >= 0;
-        at = (held ? page : 0) * a.c.n_heads + head;
+        nheld = page >= 0;
+        const int64_t at = (nheld ? page : 0) * a.c.n_heads + head;
+        page = blk + 1 < codes ? kv8_page(a.c, e.seq, blk + 1) : -1;
+        nks = a.c.k_scale[at];
+        nsv = a.c.v_scale[at];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            nk[i] = ((const i32x4 *) (a.c.k + at * BLK * D))[threadIdx.x + i * 256];
-            nv[i] = ((const i32x4 *) (a.c.v + at * BLK * D))[threadIdx.x + i * 256];
+            nk[i] = ((const i32x4 *) (a.c.k + at * BLK * D))[threadIdx.x + i * NT];
+            nv[i] = ((const i32x4 *) (a.c.v + at * BLK * D))[threadIdx.x + i * NT];
         }
     };
+    // places in a stage: of what this thread stages (piece i is NT / (D / 16) keys, NT / 4 dimensions on: the xor-ed bits stay),
+    // and of the keys and values that its lane multiplies (tile t is 4 keys on, tile d 16 dimensions: they stay, too)
+    const int pk = Stage<D>::at_k(threadIdx.x / (D / 16), threadIdx.x % (D / 16) * 2), pv = Stage<D>::at_v(threadIdx.x / 4, threadIdx.x % 4 * 2);
+    const int mk = 16 * (c >> 2) + (c & 3), mv[2] = {Stage<D>::at_v(c, 2 * g), Stage<D>::at_v(c, 2 * g + 1)};
+    int mkk[KC];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) mkk[k] = Stage<D>::at_k(mk, k * 4 + g);
+    static_assert(NT / (D / 16) % 32 == 0 && NT / 4 % 8 == 0, "pieces keep the xor-ed bits");
     auto put = [&](Stage<D> & s) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int n = threadIdx.x + i * 256;
             half8 h[2];
             to_half(nk[i], h);
-            s.k[Stage<D>::at_k(n / (D / 16), n % (D / 16) * 2)] = h[0];
-            s.k[Stage<D>::at_k(n / (D / 16), n % (D / 16) * 2 + 1)] = h[1];
+            s.k[pk + i * NT / (D / 16) * (D / 8)] = h[0];
+            s.k[(pk ^ 1) + i * NT / (D / 16) * (D / 8)] = h[1];
             to_half(nv[i], h);
-            s.v[Stage<D>::at_v(n / 4, n % 4 * 2)] = h[0];
-            s.v[Stage<D>::at_v(n / 4, n % 4 * 2 + 1)] = h[1];
+            s.v[pv + i * NT / 4 * (BLK / 8)] = h[0];
+            s.v[(pv ^ 1) + i * NT / 4 * (BLK / 8)] = h[1];
         }
-        ks = a.c.k_scale[at];
-        sv = a.c.v_scale[at];
+        held = nheld;
+        ks = nks;
+        sv = nsv;
     };
     // the tail, from its 16-bit values; bf16 is brought into the range of f16 by a power of two, as queries are
     auto put_tail = [&](Stage<D> & s) {
@@ -729,7 +748,7 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
         __syncthreads();
         float tk = 0.0f, tv = 0.0f;
         unsigned long long odd = 0;
-        for (int n = threadIdx.x; n < BLK * D / 8; n += 256) {
+        for (int n = threadIdx.x; n < BLK * D / 8; n += NT) {
             T x[8];
             load_row<T, 8>(kt + n * 8, true, x);
 #pragma unroll
@@ -756,12 +775,15 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
         __syncthreads();
         int ek = 0, ev = 0;
         if (BF) {
-            tk = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-            tv = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+#pragma unroll
+            for (int i = 0; i < MW; ++i) {
+                tk = fmaxf(tk, red[0][i]);
+                tv = fmaxf(tv, red[1][i]);
+            }
             ek = tk > 0.0f ? ilogbf(tk) : 0;
             ev = tv > 0.0f ? ilogbf(tv) : 0;
         }
-        for (int n = threadIdx.x; n < BLK * D / 8; n += 256) {
+        for (int n = threadIdx.x; n < BLK * D / 8; n += NT) {
             T x[8];
             half8 h;
             load_row<T, 8>(kt + n * 8, true, x);
@@ -823,12 +845,11 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
             floatx4 x[MR][4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const int key = 16 * (c >> 2) + 4 * t + (c & 3);
 #pragma unroll
                 for (int r = 0; r < MR; ++r) x[r][t] = floatx4{0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < KC; ++k) {
-                    const half8 kk = s.k[Stage<D>::at_k(key, k * 4 + g)];
+                    const half8 kk = s.k[mkk[k] + 4 * t * (D / 8)];
 #pragma unroll
                     for (int r = 0; r < MR; ++r) x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][k], x[r][t], 0, 0, 0);
                 }
@@ -893,7 +914,7 @@ __global__ __launch_bounds__(MW * 64, 2) void k_kv8_attend_tiles(Kv8Call a, Kv8A
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const half8 v0 = s.v[Stage<D>::at_v(d * 16 + c, 2 * g)], v1 = s.v[Stage<D>::at_v(d * 16 + c, 2 * g + 1)];
+                const half8 v0 = s.v[mv[0] + d * 16 * (BLK / 8)], v1 = s.v[mv[1] + d * 16 * (BLK / 8)];
 #pragma unroll
                 for (int r = 0; r < MR; ++r) {
                     o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, *(const half8 *) &ph[r][0], o[r][d], 0, 0, 0);
@@ -1025,7 +1046,9 @@ Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) {
     const int64_t blocks = std::max<int64_t>(1, (max_len + BLK - 1) / BLK);
     Kv8Plan plan;
     plan.many = rows > 32;
-    const int64_t tiles = plan.many ? (rows + MROWS - 1) / MROWS : (rows + 15) / 16;
+    plan.waves = 4;
+    const int mrows = plan.waves * MR * 16;
+    const int64_t tiles = plan.many ? (rows + mrows - 1) / mrows : (rows + 15) / 16;
     const int64_t groups = tiles * call.c.n_heads * call.b.n;
     int64_t per = blocks;
     // few rows: 256 parts fill the card; parts of more than 32 blocks leave it unevenly loaded where lengths differ
@@ -1033,7 +1056,7 @@ Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) {
     if (plan.many && groups < 256 && blocks > 16) per = std::max<int64_t>(8, (groups * blocks + 511) / 512);
     plan.splits = (int) ((blocks + per - 1) / per);
     plan.per = (int) ((blocks + plan.splits - 1) / plan.splits);
-    plan.tiles = (int) (plan.many ? tiles * (MROWS / 16) : tiles);
+    plan.tiles = (int) (plan.many ? tiles * (mrows / 16) : tiles);
     plan.ws_bytes = plan.splits > 1 ? (size_t) plan.tiles * call.c.n_heads * call.b.n * plan.splits * 16 * (call.c.head_dim + 2) * 4 : 0;
     // few workgroups: eight waves rather than four share a tile's blocks
     plan.wide = !plan.many && plan.splits == 1 && groups <= 256;
@@ -1042,15 +1065,18 @@ Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) {
 
 void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, const Kv8Plan & plan, int out_type) {
     const int rows = call.b.max_new * a.group;
-    const dim3 grid(plan.tiles * plan.splits, call.c.n_heads, call.b.n), join(rows, call.c.n_heads, call.b.n);
+    const int parts = plan.tiles * plan.splits;
+    const dim3 grid = parts == 1 ? dim3(1, call.c.n_heads, call.b.n) : dim3((call.c.n_heads * call.b.n + 7) / 8 * 8 * parts);
+    const dim3 join(rows, call.c.n_heads, call.b.n);
     with_type(call.c, [&](auto t, auto d) {
         using T = decltype(t);
         constexpr int D = decltype(d)::value;
         auto run = [&](auto o) {
             using O = decltype(o);
             if (plan.many) {
-                const int tiles = plan.tiles / (MROWS / 16), groups = (call.c.n_heads * call.b.n + 7) / 8 * 8;
-                OWK_LAUNCH((k_kv8_attend_tiles<T, D, O>), dim3(groups * tiles * plan.splits), dim3(MW * 64), 0, s, call, a, tiles);
+                constexpr int MW = 4;
+                const int tiles = plan.tiles / (MW * MR), groups = (call.c.n_heads * call.b.n + 7) / 8 * 8;
+                OWK_LAUNCH((k_kv8_attend_tiles<T, D, O, MW>), dim3(groups * tiles * plan.splits), dim3(MW * 64), 0, s, call, a, tiles);
             } else if (plan.wide) {
                 if (plan.tiles == 1) OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 8, true>), grid, dim3(512), 0, s, call, a);
                 else OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 8, false>), grid, dim3(512), 0, s, call, a);

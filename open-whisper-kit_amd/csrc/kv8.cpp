@@ -167,7 +167,7 @@ int owk_kv8_attend(const owk_kv8_cache * cache, const owk_kv8_batch * batch, con
     a.splits = plan.splits;
     a.per = plan.per;
     a.tiles = plan.tiles;
-    a.join = plan.many ? 8 : 1;
+    a.join = plan.many ? 2 * plan.waves : 1;
     a.scale = params->scale;
     a.ws = (float *) workspace;
     return on_device(cache->device,

@@ -71,7 +71,7 @@ struct Kv8Attend {
 
 // the split and workspace of an attend call (host arithmetic on the call's sizes alone)
 struct Kv8Plan {
-    int splits, per, tiles;
+    int splits, per, tiles, waves;
     bool many, wide;
     size_t ws_bytes;
 };

@@ -605,8 +605,8 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
 // keys 16 g .. 16 g + 15, and chunk k of eight of them is what O^T = V^T P^T wants as its k-th operand.
 // Probabilities are p = exp2(s - m) times 2^6 sv / sigma, sv the block's scale of values, sigma a power of two above it: the
 // accumulator is in units of sigma 2^-6 and the block's scale costs nothing. sigma moves (and the accumulator with it, an
-// exact step) when a scale is larger, or 2^-20 smaller and so near the end of half precision. m follows the running
-// maximum only when that has grown by more than 8: p stays below 2^8, and the accumulator is rarely rescaled.
+// exact step) when a scale is larger, or 2^-20 smaller and so near the end of half precision. m is brought up to
+// the running maximum only when a block's sum of them passes 2^14: they stay in range, and the accumulator is rarely rescaled.
 constexpr int MR = 2;  // row tiles of a wave
 
 // sixteen codes as half-precision floats: 0x6400 | x is 1024 + x
@@ -632,6 +632,22 @@ template <int D> struct Stage {
     static __device__ __forceinline__ int at_v(int d, int chunk) { return d * (BLK / 8) + (chunk ^ (d & 7)); }
 };
 
+// the entry with the n-th most tokens (of up to 64; more are taken as they come): long ones start first, short ones fill the gaps
+__device__ __forceinline__ int nth_longest(const Kv8Call & a, int n, int lane) {
+    if (a.b.n > 64) return n;
+    int len = -1;
+    if (lane < a.b.n) {
+        const Kv8Entry e = kv8_entry(a, lane);
+        len = e.start + e.n;
+    }
+    int rank = 0;
+    for (int i = 0; i < a.b.n; ++i) {
+        const int other = __builtin_amdgcn_readlane(len, i);
+        rank += other > len || (other == len && i < lane);
+    }
+    return __builtin_ctzll(__ballot(lane < a.b.n && rank == n));
+}
+
 template <typename T, int D, typename O, int MW>
 __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(Kv8Call a, Kv8Attend p, int tiles) {
     constexpr int MROWS = MW * MR * 16, NT = MW * 64;
@@ -644,9 +660,9 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     // cache; tiles that see the most keys go first
     const int id = blockIdx.x, group = (id & 7) + 8 * (id / (8 * tiles * p.splits)), rest = id / 8 % (tiles * p.splits);
     if (group >= a.c.n_heads * a.b.n) return;
-    const int head = group % a.c.n_heads, b = group / a.c.n_heads;
-    const int split = rest % p.splits, tile = tiles - 1 - rest / p.splits;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int head = group % a.c.n_heads, b = nth_longest(a, group / a.c.n_heads, lane);
+    const int split = rest % p.splits, tile = tiles - 1 - rest / p.splits;
     const Kv8Entry e = kv8_entry(a, b);
     const int nrows = e.n * p.group;
     if (tile * MROWS >= nrows) return;
@@ -701,14 +717,23 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     i32x4 nk[NC], nv[NC];
     bool held = false, nheld;  // false: block 0 of the pool is read for a block that is not there, and nothing is seen of it
     float ks = 0.0f, sv = 0.0f, nks, nsv;
-    int64_t page = lo < codes ? kv8_page(a.c, e.seq, lo) : -1;  // (a block's table entry, too, a block ahead of its codes)
+    // A block's table entry is read a block ahead of its codes, and its scales with them, by vector loads: scalar loads are
+    // counted with shared memory, and every wait for keys or values in there would wait for them, too.
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    int entry_n = -1;
+    auto ask_entry = [&](int blk) {
+        entry_n = blk < codes ? a.c.table ? a.c.table[(int64_t) e.seq * a.c.max_blocks + blk + zero] : e.seq * a.c.max_blocks + blk : -1;
+    };
+    ask_entry(lo);
     uint32_t bad = 0;   // tokens of the lane's 16 that are not finite (tail)
     auto ask = [&](int blk) {
-        nheld = page >= 0;
-        const int64_t at = (nheld ? page : 0) * a.c.n_heads + head;
-        page = blk + 1 < codes ? kv8_page(a.c, e.seq, blk + 1) : -1;
-        nks = a.c.k_scale[at];
-        nsv = a.c.v_scale[at];
+        const int page = __builtin_amdgcn_readfirstlane(entry_n);
+        nheld = page >= 0 && page < a.c.n_blocks;
+        const int64_t at = (nheld ? (int64_t) page : 0) * a.c.n_heads + head;
+        ask_entry(blk + 1);
+        nks = a.c.k_scale[at + zero];
+        nsv = a.c.v_scale[at + zero];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             nk[i] = ((const i32x4 *) (a.c.k + at * BLK * D))[threadIdx.x + i * NT];
@@ -735,8 +760,8 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
             s.v[(pv ^ 1) + i * NT / 4 * (BLK / 8)] = h[1];
         }
         held = nheld;
-        ks = nks;
-        sv = nsv;
+        ks = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(nks)));
+        sv = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(nsv)));
     };
     // the tail, from its 16-bit values; bf16 is brought into the range of f16 by a power of two, as queries are
     auto put_tail = [&](Stage<D> & s) {
@@ -808,6 +833,20 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         bad = (uint32_t) (odd_keys >> 16 * g) & 0xffff;
     };
 
+    // the scores of a staged block, in units of the block's and the rows' scales
+    auto scores = [&](const Stage<D> & s, floatx4 (&x)[MR][4]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int r = 0; r < MR; ++r) x[r][t] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                const half8 kk = s.k[mkk[k] + 4 * t * (D / 8)];
+#pragma unroll
+                for (int r = 0; r < MR; ++r) x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][k], x[r][t], 0, 0, 0);
+            }
+        }
+    };
     const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
     float m[MR], l[MR];  // the same in all four lanes of a row
     floatx4 o[MR][DT];
@@ -842,75 +881,89 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
             // what a probability is multiplied by, and what its sum is divided by
             const float mul = up == INT_MIN ? 64.0f : ldexpf(csv, 6 - sig);
             const float lg = csv == csv ? __builtin_amdgcn_logf(mul) : NAN, inv = csv == csv ? 1.0f / mul : NAN;
-            floatx4 x[MR][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                for (int r = 0; r < MR; ++r) x[r][t] = floatx4{0, 0, 0, 0};
-#pragma unroll
-                for (int k = 0; k < KC; ++k) {
-                    const half8 kk = s.k[mkk[k] + 4 * t * (D / 8)];
-#pragma unroll
-                    for (int r = 0; r < MR; ++r) x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][k], x[r][t], 0, 0, 0);
-                }
-            }
             uint32_t ph[MR][8];  // pairs of probabilities: of keys 16 g + 2 j, + 1
+            int here[MR];
+            float f[MR], by[MR];  // by: what the accumulator is multiplied by
 #pragma unroll
             for (int r = 0; r < MR; ++r) {
-                const int here = part ? there ? see[r] - base : 0 : BLK;
-                const float f = unit[r] * cks;
-                float by = moved;  // what the accumulator is multiplied by
-                // the probabilities by the m there is; where they come out too large (or there is none yet), m is brought
-                // up to the maximum and they are made again
+                here[r] = part ? there ? see[r] - base : 0 : BLK;
+                f[r] = unit[r] * cks;
+                by[r] = moved;
+            }
+            // the probabilities by the m there is, and their sum by a product with ones (what is summed is what multiplies
+            // the values); where that is too large, or there is no m yet, m is brought up to the maximum and they are made again
+            floatx4 sum[MR];
 #pragma clang loop unroll(disable)
-                for (int again = 0;; ++again) {
-                    const bool fresh = m[r] == -INFINITY;
-                    const float mm = (fresh ? 0.0f : m[r]) - lg;
-                    ushort2v big = {0, 0};  // as half-precision bits they are ordered like integers
+            for (int again = 0;; ++again) {
+                bool over = false;
+                floatx4 x[MR][4];
+                scores(s, x);
+#pragma unroll
+                for (int r = 0; r < MR; ++r) {
+                    const float mm = (m[r] == -INFINITY ? 0.0f : m[r]) - lg;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float2v y = {__builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4], f, -mm)),
-                                           __builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4 + 1], f, -mm))};
-                        const ushort2v h = __builtin_bit_cast(ushort2v, __builtin_convertvector(y, half2v));
-                        big = __builtin_elementwise_max(big, h);
-                        ph[r][j] = __builtin_bit_cast(uint32_t, h);
+                        const float2v y = {__builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4], f[r], -mm)),
+                                           __builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4 + 1], f[r], -mm))};
+                        ph[r][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, half2v));
                     }
-                    const bool over = max(big[0], big[1]) > 0x7400 /* 2^14 */ || (fresh && here > 0);
-                    if (again || !__any(over)) break;
-                    float top = -INFINITY;
-                    int till = here - 16 * g;
-                    asm volatile("" : "+v"(till));  // (keeps the comparisons in here, out of every block's way)
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) top = fmaxf(top, 4 * t + i < till ? x[r][t][i] : -INFINITY);
-                    top = max_over_g(top);
-                    const float mb = top == -INFINITY ? -INFINITY : top * f, next = fmaxf(m[r], mb);
-                    const float alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(m[r] - next);
-                    m[r] = next;
-                    l[r] *= alpha;
-                    by *= alpha;
                 }
                 if (part) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        ph[r][j] &= (16 * g + 2 * j < here ? 0xffffu : 0u) | (16 * g + 2 * j + 1 < here ? 0xffff0000u : 0u);
+                    for (int r = 0; r < MR; ++r) {
+                        int till = here[r] - 16 * g;
+                        asm volatile("" : "+v"(till));  // (keeps the masks in here, out of every block's registers)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) ph[r][j] &= (2 * j < till ? 0xffffu : 0u) | (2 * j + 1 < till ? 0xffff0000u : 0u);
+                    }
                 }
-                if (__any(by != 1.0f)) {
+#pragma unroll
+                for (int r = 0; r < MR; ++r) {
+                    sum[r] = floatx4{0, 0, 0, 0};
+                    sum[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, *(const half8 *) &ph[r][0], sum[r], 0, 0, 0);
+                    sum[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, *(const half8 *) &ph[r][4], sum[r], 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < MR; ++r) over |= sum[r][0] > 16384.0f || (m[r] == -INFINITY && here[r] > 0);
+                if (again || !__any(over)) break;
+#pragma unroll
+                for (int r = 0; r < MR; ++r) {
+                    float top = -INFINITY;
+                    int till = here[r] - 16 * g;
+                    asm volatile("" : "+v"(till) : : "memory");  // (the scores are made again rather than kept: registers)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        floatx4 y = {0, 0, 0, 0};
+#pragma unroll
+                        for (int k = 0; k < KC; ++k)
+                            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.k[mkk[k] + 4 * t * (D / 8)], q[r][k], y, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, 4 * t + i < till ? y[i] : -INFINITY);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    top = max_over_g(top);
+                    const float mb = top == -INFINITY ? -INFINITY : top * f[r], next = fmaxf(m[r], mb);
+                    const float alpha = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - next);
+                    m[r] = next;
+                    l[r] *= alpha;
+                    by[r] *= alpha;
+                }
+            }
+            if (__any(by[0] != 1.0f || by[MR - 1] != 1.0f)) {
+#pragma unroll
+                for (int r = 0; r < MR; ++r)
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[r][d][i] *= by;
-                }
-                // what is summed is what multiplies the values, by a product with ones
-                floatx4 sum = {0, 0, 0, 0};
-                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, *(const half8 *) &ph[r][0], sum, 0, 0, 0);
-                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, *(const half8 *) &ph[r][4], sum, 0, 0, 0);
-                if (here > 0) l[r] = fmaf(sum[0], inv, l[r]);
-                if (__any(cbad != 0)) {
-                    const int hit = max_over_g((int) (cbad & ((1u << min(max(here - 16 * g, 0), 16)) - 1)));
-                    if (hit) l[r] = NAN;
-                }
+                        for (int i = 0; i < 4; ++i) o[r][d][i] *= by[r];
+            }
+#pragma unroll
+            for (int r = 0; r < MR; ++r)
+                if (here[r] > 0) l[r] = fmaf(sum[r][0], inv, l[r]);
+            if (__any(cbad != 0)) {
+#pragma unroll
+                for (int r = 0; r < MR; ++r)
+                    if (max_over_g((int) (cbad & ((1u << min(max(here[r] - 16 * g, 0), 16)) - 1)))) l[r] = NAN;
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {

@@ -181,6 +181,16 @@ def check_attend(cache, model, lens, new, group, causal, layout="joined", out_ty
 # ---------------------------------------------------------------------------------------------------
 # CPU: refusals and bounds
 # ---------------------------------------------------------------------------------------------------
+class Raw:
+    """The C entries with structures passed by address (the binding itself passes packed bytes)."""
+
+    def __getattr__(self, name):
+        def call(*args):
+            return getattr(KV.load(), name)(*[C.addressof(a) if isinstance(a, C.Structure) else a for a in args])
+
+        return call
+
+
 def _desc(**kw):
     d = dict(device=0, dtype=0, head_dim=64, n_heads=2, n_seqs=3, n_blocks=12, max_blocks=4, k=4096, v=8192, k_scale=4096,
              v_scale=4096, k_tail=4096, v_tail=4096, table=None)
@@ -215,8 +225,8 @@ BAD_ROWS = [dict(data=None), dict(data=4097), dict(row=-1), dict(head=-64), dict
 
 @pytest.mark.parametrize("bad", BAD_CACHE, ids=str)
 def test_refused_caches(bad):
-    L = KV.load()
-    d = C.byref(_desc(**bad))
+    L = Raw()
+    d = _desc(**bad)
     assert L.owk_kv8_append(d, _batch(), _rows(), _rows(), None) == -1
     assert L.owk_kv8_error()
     assert L.owk_kv8_attend(d, _batch(), _params(), _rows(), _rows(), None, 0, None) == -1
@@ -226,8 +236,8 @@ def test_refused_caches(bad):
 
 @pytest.mark.parametrize("bad", BAD_BATCH, ids=str)
 def test_refused_batches(bad):
-    L = KV.load()
-    d, b = C.byref(_desc()), _batch(**bad)
+    L = Raw()
+    d, b = _desc(), _batch(**bad)
     assert L.owk_kv8_append(d, b, _rows(), _rows(), None) == -1
     assert L.owk_kv8_attend(d, b, _params(), _rows(), _rows(), None, 0, None) == -1
     assert L.owk_kv8_attend_workspace(d, b, _params()) == 0
@@ -235,8 +245,8 @@ def test_refused_batches(bad):
 
 @pytest.mark.parametrize("bad", BAD_ROWS, ids=str)
 def test_refused_tensors(bad):
-    L = KV.load()
-    d, r = C.byref(_desc()), _rows(**bad)
+    L = Raw()
+    d, r = _desc(), _rows(**bad)
     assert L.owk_kv8_append(d, _batch(), r, _rows(), None) == -1
     assert L.owk_kv8_append(d, _batch(), _rows(), r, None) == -1
     assert L.owk_kv8_attend(d, _batch(), _params(), r, _rows(), None, 0, None) == -1
@@ -247,14 +257,14 @@ def test_refused_tensors(bad):
 @pytest.mark.parametrize("bad", [dict(n_q_heads=0), dict(n_q_heads=3), dict(out_type=1), dict(out_type=3), dict(max_len=-1),
                                  dict(scale=math.inf), dict(scale=math.nan)], ids=str)
 def test_refused_params(bad):
-    L = KV.load()
-    assert L.owk_kv8_attend(C.byref(_desc()), _batch(), _params(**bad), _rows(), _rows(), None, 0, None) == -1
-    assert L.owk_kv8_attend_workspace(C.byref(_desc()), _batch(), _params(**bad)) == 0
+    L = Raw()
+    assert L.owk_kv8_attend(_desc(), _batch(), _params(**bad), _rows(), _rows(), None, 0, None) == -1
+    assert L.owk_kv8_attend_workspace(_desc(), _batch(), _params(**bad)) == 0
 
 
 def test_refused_workspaces():
-    L = KV.load()
-    d, b = C.byref(_desc(n_seqs=1, n_heads=1, n_blocks=1 << 14, max_blocks=1 << 14)), _batch(n=1, max_new=1)
+    L = Raw()
+    d, b = (_desc(n_seqs=1, n_heads=1, n_blocks=1 << 14, max_blocks=1 << 14)), _batch(n=1, max_new=1)
     need = L.owk_kv8_attend_workspace(d, b, _params(n_q_heads=1))
     if need:  # one long sequence is cut into parts
         for ws, n in ((None, 0), (4096, need - 1), (4104, need)):
@@ -263,8 +273,8 @@ def test_refused_workspaces():
 
 def test_nothing_to_do_is_no_call():
     """Empty calls succeed without a device."""
-    L = KV.load()
-    d = C.byref(_desc())
+    L = Raw()
+    d = _desc()
     for b in (_batch(n=0, lens=None), _batch(max_new=0), _batch(off=4096, rows=0)):
         assert L.owk_kv8_append(d, b, _rows(), _rows(), None) == 0
         assert L.owk_kv8_attend(d, b, _params(), _rows(), _rows(), None, 0, None) == 0
@@ -272,11 +282,11 @@ def test_nothing_to_do_is_no_call():
 
 
 def test_missing_pointers_are_refused():
-    L = KV.load()
+    L = Raw()
     assert L.owk_kv8_append(None, _batch(), _rows(), _rows(), None) == -1
-    assert L.owk_kv8_append(C.byref(_desc()), None, _rows(), _rows(), None) == -1
-    assert L.owk_kv8_append(C.byref(_desc()), _batch(), None, _rows(), None) == -1
-    assert L.owk_kv8_attend(C.byref(_desc()), _batch(), None, _rows(), _rows(), None, 0, None) == -1
+    assert L.owk_kv8_append(_desc(), None, _rows(), _rows(), None) == -1
+    assert L.owk_kv8_append(_desc(), _batch(), None, _rows(), None) == -1
+    assert L.owk_kv8_attend(_desc(), _batch(), None, _rows(), _rows(), None, 0, None) == -1
 
 
 def test_cpu_tensors_are_refused():

@@ -34,6 +34,13 @@ WHISPER_API int owk_full_batch(struct whisper_context * ctx, struct whisper_stat
                                struct whisper_full_params params, const struct owk_full_ext * ext,
                                const float * const * samples, const int * n_samples, int n_clips);
 
+/* hold the decoder's cross-attention keys and values in 8 bits (enable != 0; owk_kv8.h: a scale for each 64 frames and
+ * head) instead of f16: half the memory and traffic of what bounds a decode step. Results are close to the f16 ones, not
+ * equal. For all states of the context, from their next call on: what a state has encoded before a change is dropped, so
+ * not between whisper_encode and whisper_decode, and not while a call runs. Returns 0; -1 for a context made with
+ * dtw_token_timestamps (which read the f16 attention) or with heads of another size than 64. */
+WHISPER_API int owk_context_set_kv8(struct whisper_context * ctx, int enable);
+
 /* Silero VAD over n_streams independent streams in one device pass (all chunks encoded
  * together, one LSTM workgroup per stream, each stream from a zero state): probs_out[s]
  * receives ceil(n_samples[s] / 512) speech probabilities, the values

@@ -131,6 +131,76 @@ int set_whole_k_rows(int n) { return g_whole_k_rows.exchange(n); }
 
 void Engine::sync() { OWK_HIP_CHECK(hipStreamSynchronize(stream)); }
 
+// ---- cross K/V in 8 bits ----
+// With flash_attn the reference's cross attention covers n_ctx padded to 256 keys whose pad rows are zero (score 0, value 0):
+// the pad rows are stored as zero tokens, and a slot holds whole blocks only. soft_max attention covers n_ctx keys.
+static int kv8_blocks(const HParams & hp) { return (hp.n_audio_ctx + 255) / 256 * 256 / kKv8Block; }  // of a slot, at most
+
+static void kv8_check(int rc) {
+    if (rc) throw std::runtime_error(std::string("kv8: ") + owk_kv8_error());
+}
+
+void Engine::set_kv8(bool on) {
+    if (on == kv8_) return;
+    sync();
+    clear_graphs();
+    kv8_ = on;
+    for (DevBuf * b : {&cross_k_, &cross_v_, &kv8_k_, &kv8_v_, &kv8_ks_, &kv8_vs_, &kv8_kt_, &kv8_vt_, &kv8_fk_, &kv8_fv_, &kv8_ws_})
+        b->release();
+    cap_slots = 0;  // the next reserve() allocates the other form
+}
+
+owk_kv8_cache Engine::kv8_cache(int layer) const {
+    const HParams & hp = m->hp;
+    const size_t H = hp.n_text_head, nb = kv8_blocks(hp), blocks = (size_t) cap_slots * nb * layer, tails = (size_t) cap_slots * layer * H * kKv8Block * 64;
+    owk_kv8_cache c{};
+    c.device = m->device;
+    c.dtype = OWK_KV8_F16;
+    c.head_dim = 64;
+    c.n_heads = hp.n_text_head;
+    c.n_seqs = cap_slots;
+    c.n_blocks = (int) (cap_slots * nb);
+    c.max_blocks = (int) nb;
+    c.k = kv8_k_.as<int8_t>() + blocks * H * kKv8Block * 64;
+    c.v = kv8_v_.as<int8_t>() + blocks * H * kKv8Block * 64;
+    c.k_scale = kv8_ks_.as<float>() + blocks * H;
+    c.v_scale = kv8_vs_.as<float>() + blocks * H;
+    c.k_tail = kv8_kt_.as<_Float16>() + tails;
+    c.v_tail = kv8_vt_.as<_Float16>() + tails;
+    return c;
+}
+
+owk_kv8_attend_params Engine::kv8_params(bool f32) const {
+    owk_kv8_attend_params p{};
+    p.n_q_heads = m->hp.n_text_head;
+    p.out_type = f32 ? OWK_KV8_F32 : OWK_KV8_F16;
+    p.max_len = (n_ctx() + 255) / 256 * 256;
+    p.scale = powf(64.0f, -0.25f);  // K carries the other half of 1 / sqrt(64)
+    return p;
+}
+
+owk_kv8_batch Engine::kv8_rows(const DecShape & sh) const {
+    const char * dv = d_stg_.as<char>();
+    owk_kv8_batch b{};
+    b.n = sh.kv8_n;
+    b.max_new = sh.kv8_max;
+    b.rows = sh.R;
+    b.off = (const int32_t *) (dv + st_k8off_);
+    b.seq = (const int32_t *) (dv + st_k8seq_);
+    b.lens = (const int32_t *) (dv + st_k8len_);
+    return b;
+}
+
+// cross attention of a pass's rows over their clips' 8-bit keys and values, to f16 or f32 rows
+void Engine::kv8_cross(const DecShape & sh, int layer, hipStream_t s, const _Float16 * q, _Float16 * o16, float * o32) {
+    const int d = m->hp.n_text_state;
+    const owk_kv8_cache c = kv8_cache(layer);
+    const owk_kv8_batch b = kv8_rows(sh);
+    const owk_kv8_attend_params p = kv8_params(o32 != nullptr);
+    const owk_kv8_rows qr{const_cast<_Float16 *>(q), 0, d, 64}, outr{o32 ? (void *) o32 : (void *) o16, 0, d, 64};
+    kv8_check(owk_kv8_attend(&c, &b, &p, &qr, &outr, kv8_ws_.ptr, kv8_ws_.bytes, s));
+}
+
 void Engine::reserve(int slots, int cells) {
     const HParams & hp = m->hp;
     const size_t d = hp.n_text_state;
@@ -138,8 +208,22 @@ void Engine::reserve(int slots, int cells) {
         sync();
         cap_slots = slots;
         const size_t n = (size_t) hp.n_text_layer * cap_slots * hp.n_audio_ctx * d * 2;
-        cross_k_.alloc(n);
-        cross_v_.alloc(n);
+        if (kv8_) {
+            const size_t H = hp.n_text_head, blocks = (size_t) hp.n_text_layer * cap_slots * kv8_blocks(hp);
+            const size_t tails = (size_t) hp.n_text_layer * cap_slots * H * kKv8Block * 64 * 2;
+            for (DevBuf * b : {&kv8_k_, &kv8_v_}) b->alloc(blocks * H * kKv8Block * 64);
+            for (DevBuf * b : {&kv8_ks_, &kv8_vs_}) {
+                b->alloc(blocks * H * 4);
+                OWK_HIP_CHECK(hipMemsetAsync(b->ptr, 0, b->bytes, stream));
+            }
+            for (DevBuf * b : {&kv8_kt_, &kv8_vt_}) {
+                b->alloc(tails);
+                OWK_HIP_CHECK(hipMemsetAsync(b->ptr, 0, b->bytes, stream));
+            }
+        } else {
+            cross_k_.alloc(n);
+            cross_v_.alloc(n);
+        }
         kv_cells = 0;  // force self-KV re-allocation with the new slot count
     }
     if (cells > kv_cells) {
@@ -316,9 +400,13 @@ void Engine::encode(const std::vector<int> & slots, const std::vector<int> & off
     std::vector<MelWindow> win(n);
     for (int i = 0; i < n; ++i) win[i] = MelWindow{mel_[slots[i]]->as<float>(), mel_len_[slots[i]], offsets[i]};
     e_win_.alloc(sizeof(MelWindow) * n);
-    e_slotmap_.alloc(sizeof(int) * n);
+    // the clips' slots; for kv8 also their token counts before each append, and 64 zero values
+    std::vector<int> maps((3 * (size_t) n + 63) / 64 * 64 + 64, 0);
+    std::copy(slots.begin(), slots.end(), maps.begin());
+    std::fill(maps.begin() + 2 * n, maps.begin() + 3 * n, T);
+    e_slotmap_.alloc(sizeof(int) * maps.size());
     OWK_HIP_CHECK(hipMemcpyAsync(e_win_.ptr, win.data(), sizeof(MelWindow) * n, hipMemcpyHostToDevice, stream));
-    OWK_HIP_CHECK(hipMemcpyAsync(e_slotmap_.ptr, slots.data(), sizeof(int) * n, hipMemcpyHostToDevice, stream));
+    OWK_HIP_CHECK(hipMemcpyAsync(e_slotmap_.ptr, maps.data(), sizeof(int) * maps.size(), hipMemcpyHostToDevice, stream));
 
     auto G = [&](const char * cls, int mode, int Mr, int N, int K, const _Float16 * A, int lda, const _Float16 * W,
                  const EpiParams & ep) {
@@ -441,19 +529,45 @@ void Engine::encode(const std::vector<int> & slots, const std::vector<int> & off
     const size_t layer_stride = (size_t) cap_slots * hp.n_audio_ctx * d;  // capacity; slots of n_ctx() rows inside
     if ((uint64_t) cap_slots * T * d >= (uint64_t) 1 << 32)  // the KV_CROSS epilogue's 32-bit offsets
         throw std::runtime_error("encode: cross K/V offsets exceed 32 bits");
+    if (kv8_) {
+        if (hp.n_text_state != hp.n_text_head * 64) throw std::runtime_error("encode: kv8 needs heads of 64");
+        if (kv8_fk_.bytes < (size_t) M * d * 2) {
+            sync();
+            kv8_fk_.alloc((size_t) M * d * 2);
+            kv8_fv_.alloc((size_t) M * d * 2);
+        }
+    }
     for (int l = 0; l < hp.n_text_layer; ++l) {
         const DecLayerW & L = m->dec[l];
         EpiParams ep;
         ep.scale = k_scale;
         ep.bias2 = L.cb_v;
-        ep.out16b = cross_k_.as<_Float16>() + l * layer_stride;
-        ep.out16c = cross_v_.as<_Float16>() + l * layer_stride;
+        ep.out16b = kv8_ ? kv8_fk_.as<_Float16>() : cross_k_.as<_Float16>() + l * layer_stride;
+        ep.out16c = kv8_ ? kv8_fv_.as<_Float16>() : cross_v_.as<_Float16>() + l * layer_stride;
         ep.d = d;
         ep.T = T;
-        ep.slot_map = e_slotmap_.as<int>();
+        ep.slot_map = kv8_ ? nullptr : e_slotmap_.as<int>();
         // Q5_0: the final LayerNorm wrote the encoder output's Q8_0 rows once for all layers
         linear("gemm_cross", EPI_KV_CROSS, M, 2 * d, d, e_enc_.as<_Float16>(), m->q5 ? e_enc32_.as<float>() : nullptr, d,
                L.cw_kv, L.q_ckv, ep, nullptr, false, m->q5 && !m->kq);
+        if (kv8_) {
+            ProfScope ps(prof, stream, "kv8_append", 0, 2.0 * M * (double) d * 3);
+            const owk_kv8_cache c = kv8_cache(l);
+            owk_kv8_batch bt{};
+            bt.n = n;
+            bt.max_new = T;
+            bt.seq = e_slotmap_.as<int>();
+            bt.lens = e_slotmap_.as<int>() + n;  // zeros
+            owk_kv8_rows kr{kv8_fk_.ptr, (int64_t) T * d, 64, (int64_t) T * 64}, vr = kr;
+            vr.data = kv8_fv_.ptr;
+            kv8_check(owk_kv8_append(&c, &bt, &kr, &vr, stream));
+            if (flash_attn && n_zero_pad > 0) {
+                bt.max_new = n_zero_pad;
+                bt.lens = e_slotmap_.as<int>() + 2 * n;  // n_ctx()
+                const owk_kv8_rows zr{e_slotmap_.as<char>() + ((size_t) 3 * n * 4 + 255) / 256 * 256, 0, 0, 0};  // one row of zeros
+                kv8_check(owk_kv8_append(&c, &bt, &zr, &zr, stream));
+            }
+        }
     }
     kq_rmul_ = nullptr;
 }
@@ -470,6 +584,21 @@ void Engine::download_cross(int slot, int layer, uint16_t * kh, uint16_t * vh) c
     OWK_HIP_CHECK(hipStreamSynchronize(stream));
     const int T = n_ctx(), d = hp.n_text_state, H = d / 64;
     const size_t per = (size_t) T * d;
+    if (kv8_) {
+        if (slot < 0 || slot >= cap_slots || layer < 0 || layer >= hp.n_text_layer) throw std::runtime_error("download_cross: no such slot");
+        const int zl[2] = {flash_attn ? (T + 255) / 256 * 256 : T, slot};  // tokens the slot holds, its sequence
+        DevBuf out, idx;
+        out.alloc(2 * per * 2);
+        idx.alloc(sizeof(zl));
+        OWK_HIP_CHECK(hipMemcpy(idx.ptr, zl, sizeof(zl), hipMemcpyHostToDevice));
+        const owk_kv8_cache c = kv8_cache(layer);
+        const owk_kv8_rows kr{out.ptr, 0, d, 64}, vr{out.as<_Float16>() + per, 0, d, 64};
+        kv8_check(owk_kv8_read(&c, 1, T, idx.as<int>(), idx.as<int>() + 1, nullptr, &kr, &vr, stream));
+        OWK_HIP_CHECK(hipStreamSynchronize(stream));
+        OWK_HIP_CHECK(hipMemcpy(kh, out.ptr, per * 2, hipMemcpyDeviceToHost));
+        OWK_HIP_CHECK(hipMemcpy(vh, out.as<_Float16>() + per, per * 2, hipMemcpyDeviceToHost));
+        return;
+    }
     const size_t o = (size_t) layer * cap_slots * hp.n_audio_ctx * d + (size_t) slot * per;
     // device layout is head-major [head][t][64]; the caller gets the reference's [t][d]
     std::vector<uint16_t> tk(per), tv(per);
@@ -499,6 +628,9 @@ void Engine::stage_layout(int C, int KC) {
     st_rc_ = sec((size_t) C * sizeof(AttnRow));
     st_lsel_ = sec((size_t) C * 4);
     st_rmul_ = sec((size_t) C);
+    st_k8off_ = sec((size_t) (C + 1) * 4);
+    st_k8seq_ = sec((size_t) C * 4);
+    st_k8len_ = sec((size_t) C * 4);
     st_keys_ = sec((size_t) KC * 4);
     st_bytes_ = o;
 }
@@ -515,7 +647,8 @@ uint64_t Engine::buffers_signature() const {
     uint64_t h = 1469598103934665603ull;
     for (const void * p : {d_x_.ptr, d_xn_.ptr, d_q_.ptr, d_ao_.ptr, d_h_.ptr, d_xl_.ptr, logits_.ptr, d_stg_.ptr,
                            q8a_.ptr, q8d_.ptr, q8h_.ptr, q8hd_.ptr, d_xn32_.ptr, d_ao32_.ptr, d_xl32_.ptr, q16a_.ptr, q16d_.ptr,
-                           self_k_.ptr, self_v_.ptr, cross_k_.ptr, cross_v_.ptr, gws_part_.ptr, sm_ws_.ptr})
+                           self_k_.ptr, self_v_.ptr, cross_k_.ptr, cross_v_.ptr, gws_part_.ptr, sm_ws_.ptr, kv8_k_.ptr, kv8_v_.ptr,
+                           kv8_ks_.ptr, kv8_vs_.ptr, kv8_kt_.ptr, kv8_vt_.ptr, kv8_ws_.ptr})
         h = (h ^ (uint64_t) (uintptr_t) p) * 1099511628211ull;
     return h;
 }
@@ -633,6 +766,27 @@ void Engine::decode(const std::vector<DecodeRow> & rows, const std::vector<int> 
         std::sort(slots.begin(), slots.end());
         sh.n_clips = (int) (std::unique(slots.begin(), slots.end()) - slots.begin());
     }
+    if (kv8_) {
+        int * off = (int *) (h + st_k8off_), * seq = (int *) (h + st_k8seq_), * len = (int *) (h + st_k8len_);
+        for (int r = 0; r < R; ++r) {
+            if (r && rows[r].slot == rows[r - 1].slot) continue;
+            off[sh.kv8_n] = r;
+            seq[sh.kv8_n] = rows[r].slot;
+            len[sh.kv8_n] = flash_attn ? n_ctx_pad : T;
+            if (sh.kv8_n) sh.kv8_max = std::max(sh.kv8_max, r - off[sh.kv8_n - 1]);
+            sh.kv8_n++;
+        }
+        off[sh.kv8_n] = R;
+        sh.kv8_max = std::max(sh.kv8_max, R - off[sh.kv8_n - 1]);
+        const owk_kv8_cache c = kv8_cache(0);
+        const owk_kv8_batch b = kv8_rows(sh);
+        const owk_kv8_attend_params p = kv8_params(m->q5);
+        const size_t need = owk_kv8_attend_workspace(&c, &b, &p);
+        if (need > kv8_ws_.bytes) {
+            sync();
+            kv8_ws_.alloc(need);
+        }
+    }
     if (m->kq && qf_k_repacked(m->qfmt)) {
         // each clip's rows of this pass are one reference decode batch (its decoders' tokens, or a
         // prompt): the rows of its complete groups of 4 take the repack quantizer
@@ -658,6 +812,7 @@ void Engine::decode(const std::vector<DecodeRow> & rows, const std::vector<int> 
         OWK_HIP_CHECK(hipMemsetAsync(sm_ws_.ptr, 0, sm_ws_.bytes, stream));  // arrival tickets start at 0
     }
     if (capture) {
+        if (kv8_) throw std::runtime_error("decode: capture needs the f16 cross K/V");
         if (!n_ah_ || !amap_.ptr) throw std::runtime_error("decode: capture without alignment heads");
         if (!sh.cross_sm) throw std::runtime_error("decode: capture needs soft_max cross attention (flash_attn = false)");
         cap_.alloc((size_t) n_ah_ * T * R * 4);
@@ -682,11 +837,12 @@ void Engine::decode(const std::vector<DecodeRow> & rows, const std::vector<int> 
                            ((uint64_t) sh.self_sm << 44) | ((uint64_t) sh.cross_sm << 45) |
                            ((uint64_t) sh.self_list << 46) | ((uint64_t) (R <= whole_k_rows()) << 47) |
                            ((uint64_t) T << 48);
-    const uint64_t key = (uint64_t) R | ((uint64_t) n_logit_rows << 20) | shape;
+    const std::pair<uint64_t, uint64_t> key((uint64_t) R | ((uint64_t) n_logit_rows << 20) | shape,
+                                            (uint64_t) sh.kv8_n | ((uint64_t) sh.kv8_max << 32));
     OWK_HIP_CHECK(hipGraphLaunch(graph_for(key, stream, [&]() { launch_decode(sh); }), stream));
 }
 
-hipGraphExec_t Engine::graph_for(uint64_t key, hipStream_t s, const std::function<void()> & launch) {
+hipGraphExec_t Engine::graph_for(const std::pair<uint64_t, uint64_t> & key, hipStream_t s, const std::function<void()> & launch) {
     auto it = graphs_.find(key);
     if (it != graphs_.end()) return it->second;
     if (graphs_.size() >= 64) clear_graphs();
@@ -747,7 +903,7 @@ void Engine::launch_decode(const DecShape & sh) {
     const bool kq = m->kq;  // K-quants: GEMMs quantize f32 rows to Q8_K themselves (no producer rows)
     kq_rmul_ = kq && qf_k_repacked(m->qfmt) ? (const uint8_t *) (dv + st_rmul_) : nullptr;
     const bool fq_self = q5 && !kq && self_oc && !self_tl && !sh.self_sm;
-    const bool fq_cross = q5 && !kq && cross_oc && !cross_tl && !sh.cross_sm;
+    const bool fq_cross = q5 && !kq && cross_oc && !cross_tl && !sh.cross_sm && !kv8_;
     float * xn32 = kq ? d_xn32_.as<float>() : nullptr;  // the f32 LayerNorm rows a K-quant GEMM quantizes
 
     {
@@ -761,6 +917,10 @@ void Engine::launch_decode(const DecShape & sh) {
     const size_t cross_stride = (size_t) cap_slots * hp.n_audio_ctx * d;  // per layer (capacity)
     // one_chunk / tiled cross attention of layer l (soft_max rows: attn_decoder_softmax at the call site)
     auto cross_attn = [&](int l, const _Float16 * qv, _Float16 * o16, float * o32, int8_t * q8, float * q8d) {
+        if (kv8_) {
+            kv8_cross(sh, l, stream, qv, o16, o32);
+            return;
+        }
         attn_decoder(stream, qv, d, cross_k_.as<_Float16>() + l * cross_stride, cross_v_.as<_Float16>() + l * cross_stride,
                      64, T * 64, d_rc, R, nullptr, H, kq_scale, T, o16, d, cross_oc, cross_tl, o32, true, q8, q8d);
     };
@@ -829,7 +989,7 @@ void Engine::launch_decode(const DecShape & sh) {
             G("cq", EPI_F16, d, d, d_xn_.as<_Float16>(), nullptr, L.cw_q, L.t_cq, L.q_cq, ep, R, true);
         }
         {
-            ProfScope ps(prof, stream, "attn_cross", 4.0 * R * (double) n_ctx_pad * d, 2.0 * 2.0 * sh.n_clips * (double) T * d);
+            ProfScope ps(prof, stream, "attn_cross", 4.0 * R * (double) n_ctx_pad * d, (kv8_ ? 1.0 : 2.0) * 2.0 * sh.n_clips * (double) T * d);
             cross_attn(l, d_q_.as<_Float16>(), d_ao_.as<_Float16>(), fq_cross ? nullptr : ao32, fq_cross ? q8a() : nullptr,
                        fq_cross ? q8d() : nullptr);
         }
@@ -890,10 +1050,10 @@ void Engine::launch_decode(const DecShape & sh) {
         }
         {
             // bytes: cross K and V of each row's clip (the HBM-bound part of a decode step)
-            ProfScope ps(prof, stream, "attn_cross", 4.0 * R * (double) n_ctx_pad * d, 2.0 * 2.0 * sh.n_clips * (double) T * d);
+            ProfScope ps(prof, stream, "attn_cross", 4.0 * R * (double) n_ctx_pad * d, (kv8_ ? 1.0 : 2.0) * 2.0 * sh.n_clips * (double) T * d);
             cross_attn(l, d_q_.as<_Float16>(), d_ao_.as<_Float16>(), fq_cross ? nullptr : ao32, fq_cross ? q8a() : nullptr,
                        fq_cross ? q8d() : nullptr);
-            if (sh.cross_sm)  // soft_max_ext(KQ, nullptr, KQscale) over n_audio_ctx keys (whisper.cpp:2697-2738)
+            if (sh.cross_sm && !kv8_)  // soft_max_ext(KQ, nullptr, KQscale) over n_audio_ctx keys (whisper.cpp:2697-2738)
                 attn_decoder_softmax(stream, d_q_.as<_Float16>(), d, cross_k_.as<_Float16>() + l * cross_stride,
                                      cross_v_.as<_Float16>() + l * cross_stride, 64, T * 64, d_rc, R, nullptr, H, kq_scale, T,
                                      d_ao_.as<_Float16>(), d, sh.capture ? amap_.as<int>() + l * H : nullptr,
@@ -1038,10 +1198,11 @@ void Engine::fused_part(const DecShape & sh, int r0, int n, hipStream_t s, const
             consumer(EPI_F16, d, L.cross_ln_w, L.cross_ln_b, L.t_cq, ep, 0);
         }
         {
-            ProfScope ps(prof, s, "attn_cross", 4.0 * n * (double) n_ctx_pad * d, 2.0 * 2.0 * sh.n_clips * (double) T * d);
-            attn_decoder(s, q_abs, d, Kc, Vc, 64, T * 64, d_rc, n, nullptr, H, kq_scale, T, ao_abs, d, sh.cross_oc,
-                         sh.cross_tl, nullptr, true, nullptr, nullptr);
-            if (sh.cross_sm)  // soft_max_ext over n_audio_ctx keys (key-split), DTW capture of the alignment heads
+            ProfScope ps(prof, s, "attn_cross", 4.0 * n * (double) n_ctx_pad * d, (kv8_ ? 1.0 : 2.0) * 2.0 * sh.n_clips * (double) T * d);
+            if (kv8_) kv8_cross(sh, l, s, q_abs, ao_abs, nullptr);
+            else attn_decoder(s, q_abs, d, Kc, Vc, 64, T * 64, d_rc, n, nullptr, H, kq_scale, T, ao_abs, d, sh.cross_oc,
+                              sh.cross_tl, nullptr, true, nullptr, nullptr);
+            if (sh.cross_sm && !kv8_)  // soft_max_ext over n_audio_ctx keys (key-split), DTW capture of the alignment heads
                 attn_decoder_softmax(s, q_abs, d, Kc, Vc, 64, T * 64, d_rc, n, nullptr, H, kq_scale, T, ao_abs, d,
                                      sh.capture ? amap_.as<int>() + l * H : nullptr,
                                      sh.capture ? cap_.as<float>() : nullptr, sh.R, nullptr, smw, smw_floats);

@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "kv8.h"
 #include "model.h"
 
 namespace owk {
@@ -79,6 +80,7 @@ struct DecShape {
     bool self_sm = false, cross_sm = false;     // soft_max rows (flash_attn = false contexts)
     bool capture = false;                       // DTW: capture alignment-head cross-attention
     bool self_list = false;                     // a one_chunk self row whose cells are not one run
+    int kv8_n = 0, kv8_max = 0;                 // kv8: runs of rows of one clip, and the rows of the longest
     int n_clips = 0;                            // distinct clips (cross K/V slots) among the rows: the
                                                 // cross K/V a pass must read is per clip, not per row
 };
@@ -108,6 +110,8 @@ public:
     // 6986): 0 = the model's n_audio_ctx. The encoder runs over n_ctx() positions (2 * n_ctx() mel
     // frames), cross K/V hold n_ctx() rows per slot and decoder cross-attention attends over them.
     int audio_ctx = 0;
+    // owk_context_set_kv8: the cross K/V held in 8 bits (owk_kv8.h) instead of f16; drops what is cached when it changes
+    void set_kv8(bool on);
     int n_ctx() const { return audio_ctx > 0 && audio_ctx < m->hp.n_audio_ctx ? audio_ctx : m->hp.n_audio_ctx; }
 
     void reserve(int slots, int cells);
@@ -171,6 +175,15 @@ private:
     DevBuf post_d_, post_out_d_;
     // slot storage
     DevBuf cross_k_, cross_v_;   // [L][cap_slots][n_audio_ctx][d]
+    bool kv8_ = false;
+    DevBuf kv8_k_, kv8_v_;       // kv8_: codes [L][cap_slots][blocks][head][64 * 64], and their scales and tails
+    DevBuf kv8_ks_, kv8_vs_, kv8_kt_, kv8_vt_;
+    DevBuf kv8_fk_, kv8_fv_;     // one layer's f16 K/V of an encode call [clip][head][n_ctx][64], on their way to codes
+    DevBuf kv8_ws_;
+    owk_kv8_cache kv8_cache(int layer) const;
+    owk_kv8_attend_params kv8_params(bool f32) const;
+    owk_kv8_batch kv8_rows(const DecShape & sh) const;
+    void kv8_cross(const DecShape & sh, int layer, hipStream_t s, const _Float16 * q, _Float16 * o16, float * o32);
     DevBuf self_k_, self_v_;     // [L][cap_slots][head][kv_cells][64] (head-major)
     std::vector<DevBuf *> mel_;  // per slot [n_mel][n_len]
     std::vector<int> mel_len_;
@@ -191,10 +204,11 @@ private:
     PinnedBuf stg_;   // host image of the per-pass inputs
     DevBuf d_stg_;    // its device copy (fixed sections, see stage_layout)
     size_t st_tok_ = 0, st_pos_ = 0, st_rowoff_ = 0, st_rs_ = 0, st_rc_ = 0, st_lsel_ = 0, st_keys_ = 0, st_bytes_ = 0;
+    size_t st_k8off_ = 0, st_k8seq_ = 0, st_k8len_ = 0;  // kv8: the pass's rows by clip (owk_kv8_batch)
     size_t st_rmul_ = 0;  // K-quants (repacked formats): per-row Q8_K rounding path (quantize_q8k_f16)
-    std::map<uint64_t, hipGraphExec_t> graphs_;
+    std::map<std::pair<uint64_t, uint64_t>, hipGraphExec_t> graphs_;
     uint64_t graphs_sig_ = 0;
-    hipGraphExec_t graph_for(uint64_t key, hipStream_t s, const std::function<void()> & launch);
+    hipGraphExec_t graph_for(const std::pair<uint64_t, uint64_t> & key, hipStream_t s, const std::function<void()> & launch);
 
     // Q5_0 models: f32 activations feeding the quantized GEMMs and their Q8_0 copy
     void linear(const char * cls, int mode, int M, int N, int K, const _Float16 * A16, const float * A32, int lda,

@@ -93,6 +93,7 @@ struct whisper_context {
     std::unique_ptr<owk::Model> model;
     whisper_state * state = nullptr;
     std::string path_model;
+    bool kv8 = false;  // owk_context_set_kv8
     owk::Prof prof;
     std::mutex mu;  // whisper_full calls while the per-kernel recorder (prof, shared) is on
     whisper_timings timings{};

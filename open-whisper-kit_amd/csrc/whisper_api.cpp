@@ -238,6 +238,7 @@ bool alignment_heads(const whisper_context * ctx, std::vector<int> & amap, int &
 void configure_engine(const whisper_context * ctx, whisper_state * st) {
     if (!st->eng) return;
     st->eng->flash_attn = ctx->params.flash_attn;
+    st->eng->set_kv8(ctx->kv8);
     if (ctx->params.dtw_token_timestamps && st->dtw_n_ah > 0 && st->eng->n_aheads() == 0)
         st->eng->set_alignment_heads(st->dtw_amap, st->dtw_n_ah);
 }
@@ -1199,6 +1200,20 @@ int owk_debug_enc(struct whisper_context * ctx, struct whisper_state * st, int i
         st->eng->download_enc(index, out);
     }
     return n;
+}
+
+int owk_context_set_kv8(struct whisper_context * ctx, int enable) {
+    if (!ctx) return -1;
+    if (enable && ctx->params.dtw_token_timestamps) {
+        log_msg(GGML_LOG_LEVEL_ERROR, "%s: DTW timestamps read the f16 cross attention\n", __func__);
+        return -1;
+    }
+    if (enable && ctx->model->hp.n_text_state != 64 * ctx->model->hp.n_text_head) {
+        log_msg(GGML_LOG_LEVEL_ERROR, "%s: heads of 64 are needed\n", __func__);
+        return -1;
+    }
+    ctx->kv8 = enable != 0;
+    return 0;
 }
 
 int owk_debug_cross(struct whisper_context * ctx, struct whisper_state * st, int slot, int layer, uint16_t * k, uint16_t * v) {

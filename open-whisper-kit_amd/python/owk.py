@@ -193,6 +193,7 @@ def load(path: str | None = None) -> C.CDLL:
     L.whisper_lang_auto_detect_with_state.argtypes = [vp, vp, ip, ip, fp]
     L.whisper_lang_max_id.restype = ip
     L.whisper_log_set.argtypes = [vp, vp]
+    L.owk_context_set_kv8.argtypes = [vp, ip]
     L.owk_prof_enable.argtypes = [vp, ip]
     L.owk_prof_select.argtypes = [vp, C.c_char_p]
     L.owk_prof_reset.argtypes = [vp]
@@ -262,7 +263,7 @@ class Whisper:
     """Thin owner of a whisper_context (and its default state)."""
 
     def __init__(self, model_path: str, device: int = 0, flash_attn: bool = True, dtw_preset: int = 0,
-                 dtw_n_top: int = -1):
+                 dtw_n_top: int = -1, kv8: bool = False):
         self.L = load()
         cp = self.L.whisper_context_default_params()
         cp.gpu_device = device
@@ -275,6 +276,10 @@ class Whisper:
         self.ctx = self.L.whisper_init_from_file_with_params(model_path.encode(), cp)
         if not self.ctx:
             raise RuntimeError(f"whisper_init_from_file_with_params failed for {model_path}")
+        if kv8 and self.L.owk_context_set_kv8(self.ctx, 1) != 0:
+            self.L.whisper_free(self.ctx)
+            self.ctx = None
+            raise ValueError("this context cannot hold its cross keys and values in 8 bits (DTW timestamps, or heads not of 64)")
         self.n_vocab = self.L.whisper_n_vocab(self.ctx)
         self._states = []
 

@@ -38,6 +38,15 @@ __device__ __forceinline__ float wave_sum(float x) {
     return x;
 }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// The quotient is rounded once and the code once: a quotient by the reciprocal would move codes at ties. A block without a
+// finite scale has zeros (and reads as NaN), and one of zeros, too.
+__device__ __forceinline__ int8_t code_of(float x, float scale) {
+    const float y = scale > 0.0f ? rintf(x / scale) : 0.0f;
+    return (int8_t) fminf(fmaxf(y, -127.0f), 127.0f);
+}
+
 // N elements of a row, as vectors where the tensor allows it
 template <typename T, int N> __device__ __forceinline__ void load_row(const T * p, bool vec, T (&x)[N]) {
     if (vec) {
@@ -106,15 +115,12 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8Call a, Kv8Rows kr, Kv8Ro
         if ((threadIdx.x & 63) == 0) amax[threadIdx.x >> 6] = m;
         __syncthreads();
         m = fmaxf(fmaxf(amax[0], amax[1]), fmaxf(amax[2], amax[3]));
-        const bool whole = m <= 3.402823466e38f;
-        const float scale = whole ? m / 127.0f : NAN;
+        const float scale = finite(m) ? m / 127.0f : NAN;
         const int64_t page = kv8_page(a.c, e.seq, blk);
         alignas(16) int8_t c[Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-            // the quotient is rounded once and the code once: a quotient by the reciprocal would move codes at ties
-            const float y = whole && scale > 0.0f ? rintf(to_f32(x[i]) / scale) : 0.0f;
-            c[i] = (int8_t) fminf(fmaxf(y, -127.0f), 127.0f);
+            c[i] = code_of(to_f32(x[i]), scale);
         }
         if (page >= 0) {
             if (threadIdx.x == 0) (is_v ? a.c.v_scale : a.c.k_scale)[page * a.c.n_heads + head] = scale;
@@ -163,7 +169,10 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Call a, const int32_t * fir
     const int first = first_of ? max(first_of[b], 0) : 0;
     const int64_t blk = (int64_t) first / BLK + blockIdx.x;
     const int t = threadIdx.x / 4, d0 = (threadIdx.x % 4) * Q;
-    __shared__ __align__(16) int8_t tile[BLK * PITCH];
+    __shared__ __align__(16) char store[BLK * (D + 2) * sizeof(T)];
+    int8_t * tile = (int8_t *) store;  // [token][PITCH] codes
+    T * half = (T *) store;            // [token][D + 2] values of the tail
+    static_assert(BLK * PITCH <= sizeof(store), "both forms fit");
     T x[Q];
 #pragma unroll
     for (int k = 0; k < Q; ++k) x[k] = (T) 0.0f;
@@ -171,9 +180,16 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Call a, const int32_t * fir
     if (e.seq >= 0 && blk * BLK < e.start) {
         if (blk == e.start / BLK) {
             const T * tail = (const T *) (is_v ? a.c.v_tail : a.c.k_tail) + ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
-            if (held && is_v) {
+            if (is_v) {
+                for (int i = threadIdx.x; i < D * 8; i += 256) {
+                    T z[8];
+                    load_row<T, 8>(tail + i * 8, true, z);
 #pragma unroll
-                for (int k = 0; k < Q; ++k) x[k] = tail[(d0 + k) * BLK + t];
+                    for (int k = 0; k < 8; ++k) half[(i % 8 * 8 + k) * (D + 2) + i / 8] = z[k];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < Q; ++k) x[k] = held ? half[t * (D + 2) + d0 + k] : (T) 0.0f;
             } else if (held) {
                 load_row<T, Q>(tail + t * D + d0, true, x);
             }
@@ -246,7 +262,6 @@ __device__ __forceinline__ float sum_over_g(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // The two bytes of four values in [-1, 1]. A float of 1.5 * 2^23 + z has the integer z in its low bits, so one fma rounds
 // to the unit; with z = value + 128, byte 1 of z is hi and byte 0 of it is lo + 128.
@@ -293,8 +308,8 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     // values, dimension-major: lane (c, g) reads keys 16 g .. 16 g + 15 of dimension 16 dt + c
     // (asked for before the scores where the registers allow it)
-    auto values = [&](int dt, int k) { return *(const vec8 *) (vt + (dt * 16 + c) * BLK + 16 * g + 8 * k); };
-    vec8 vx[D == 64 ? 4 : 1][2];
+    auto values = [&](int dt, int k) { return *(const u32x4 *) (vt + (dt * 16 + c) * BLK + 16 * g + 8 * k); };
+    u32x4 vx[D == 64 ? 4 : 1][2];
     if (D == 64)
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
@@ -316,8 +331,8 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
             floatx4 x = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
-                vec8 k = {};
-                if (key < have) k = *(const vec8 *) (kt + key * D + j * 32 + g * 8);
+                // (behind the last token its own row again: the score is hidden below)
+                const vec8 k = *(const vec8 *) (kt + min(key, have - 1) * D + j * 32 + g * 8);
                 x = mfma16(k, q[j], x);
             }
 #pragma unroll
@@ -351,20 +366,40 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
     if (!BF) ls *= 1.0f / 16384.0f;
     uint32_t bad = 0;  // of the lane's 16 keys
     const float fo = BF ? f : f * (1.0f / 16384.0f);
+    u32x4 keep[2];  // pairs of the lane's keys: those that are there
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = 16 * g + 8 * k + 2 * i;
+            keep[k][i] = (key < have ? 0xffffu : 0u) | (key + 1 < have ? 0xffff0000u : 0u);
+        }
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
+        u32x4 v[2];
+        ushort2v big = {0, 0};  // magnitudes as bits: what is not finite is on top
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            v[k] = (D == 64 ? vx[D == 64 ? dt : 0][k] : values(dt, k)) & keep[k];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(ushort2v, v[k][i] & 0x7fff7fffu));
+        }
+        constexpr uint32_t INF = BF ? 0x7f80 : 0x7c00;
+        if (__any(max(big[0], big[1]) >= INF)) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool lo = (v[k][i] & 0x7fffu) >= INF, hi = (v[k][i] >> 16 & 0x7fffu) >= INF;
+                    bad |= (lo ? 1u : 0u) << (8 * k + 2 * i) | (hi ? 2u : 0u) << (8 * k + 2 * i);
+                    v[k][i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                }
+        }
         floatx4 x = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            vec8 v = D == 64 ? vx[D == 64 ? dt : 0][k] : values(dt, k);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool mine = 16 * g + 8 * k + i < have, fine = finite(to_f32(v[i]));
-                bad |= mine && !fine ? 1u << (8 * k + i) : 0u;
-                v[i] = mine && fine ? v[i] : (T) 0.0f;
-            }
-            x = mfma16(v, ph[k], x);
-            if (BF) x = mfma16(v, pl[k], x);
+            x = mfma16(__builtin_bit_cast(vec8, v[k]), ph[k], x);
+            if (BF) x = mfma16(__builtin_bit_cast(vec8, v[k]), pl[k], x);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc.o[dt][i] = fmaf(x[i], fo, acc.o[dt][i] * alpha);

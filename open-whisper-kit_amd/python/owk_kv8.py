@@ -213,7 +213,7 @@ class Cache:
         if seq is None and n > self.n_seqs:
             raise ValueError(f"{n} entries, and the cache has {self.n_seqs} sequences")
         h, d = self.n_heads, self.head_dim
-        kv = torch.empty((2, n, max_tokens, h, d), dtype=self.dtype, device=self.device)
+        kv = self.k_tail.new_empty((2, n, max_tokens, h, d))
         k, v = kv.unbind(0)
         i = self._index("lens", lens, n), self._index("seq", seq, n), self._index("first", first, n)
         if kv.numel():

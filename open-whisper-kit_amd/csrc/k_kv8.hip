@@ -412,6 +412,24 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
     acc.l += f * ls;
 }
 
+// Which entry and head (group) a workgroup of a one-dimensional grid works on, and which of its `parts` parts. Workgroups go
+// round the eight dies: all parts of a group run on one die, and the keys they share stay in its cache (32 groups of 128-row
+// tiles: 345 us, 405 without), unless that would leave the dies unevenly loaded (4 groups of 62 parts: 35 us, 22 without).
+__host__ __device__ inline bool by_die(int groups) { return (groups + 7) / 8 * 56 <= groups * 8; }
+struct Place {
+    int group, part;  // group -1: nothing to do
+};
+__device__ __forceinline__ Place place_of(const Kv8Call & a, int parts) {
+    const int id = blockIdx.x, groups = a.c.n_heads * a.b.n;
+    if (!by_die(groups)) return Place{id / parts, id % parts};
+    const int group = (id & 7) + 8 * (id / (8 * parts));
+    return Place{group < groups ? group : -1, id / 8 % parts};
+}
+unsigned workgroups(const Kv8Call & call, int parts) {
+    const unsigned groups = (unsigned) call.c.n_heads * call.b.n;
+    return (by_die(groups) ? (groups + 7) / 8 * 8 : groups) * parts;
+}
+
 // ONCE: no other tile reads these codes, they need not stay in the caches (cross attention of 32 clips 29.3 -> 26.7 us;
 // with more tiles of the same keys 141 -> 171 us, so then it is off)
 template <bool ONCE> __device__ __forceinline__ i32x4 load_codes(const int8_t * p) {
@@ -421,16 +439,14 @@ template <bool ONCE> __device__ __forceinline__ i32x4 load_codes(const int8_t * 
 template <typename T, int D, typename O, int W, bool ONCE>
 __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8Call a, Kv8Attend p) {
     constexpr int DT = D / 16, KC = D / 64;
-    // the tiles of one entry and head run on one of the eight dies (workgroups go round them): the keys they share stay in
-    // its cache
     int head = blockIdx.y, b = blockIdx.z, split = 0, tile = 0;
     if (gridDim.x > 1) {
-        const int id = blockIdx.x, group = (id & 7) + 8 * (id / (8 * p.tiles * p.splits)), rest = id / 8 % (p.tiles * p.splits);
-        if (group >= a.c.n_heads * a.b.n) return;
-        head = group % a.c.n_heads;
-        b = group / a.c.n_heads;
-        split = rest % p.splits;
-        tile = rest / p.splits;
+        const Place place = place_of(a, p.tiles * p.splits);
+        if (place.group < 0) return;
+        head = place.group % a.c.n_heads;
+        b = place.group / a.c.n_heads;
+        split = place.part % p.splits;
+        tile = place.part / p.splits;
     }
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const Kv8Entry e = kv8_entry(a, b);
@@ -691,13 +707,11 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     __shared__ __align__(16) Stage<D> st[2];
     __shared__ float red[2][MW];
     __shared__ unsigned long long odd_keys;
-    // the tiles of one entry and head run on one of the eight dies (workgroups go round them): their keys stay in its
-    // cache; tiles that see the most keys go first
-    const int id = blockIdx.x, group = (id & 7) + 8 * (id / (8 * tiles * p.splits)), rest = id / 8 % (tiles * p.splits);
-    if (group >= a.c.n_heads * a.b.n) return;
+    const Place place = place_of(a, tiles * p.splits);
+    if (place.group < 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    const int head = group % a.c.n_heads, b = nth_longest(a, group / a.c.n_heads, lane);
-    const int split = rest % p.splits, tile = tiles - 1 - rest / p.splits;
+    const int head = place.group % a.c.n_heads, b = nth_longest(a, place.group / a.c.n_heads, lane);
+    const int split = place.part % p.splits, tile = tiles - 1 - place.part / p.splits;  // tiles that see the most keys first
     const Kv8Entry e = kv8_entry(a, b);
     const int nrows = e.n * p.group;
     if (tile * MROWS >= nrows) return;
@@ -1154,7 +1168,7 @@ Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) {
 void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, const Kv8Plan & plan, int out_type) {
     const int rows = call.b.max_new * a.group;
     const int parts = plan.tiles * plan.splits;
-    const dim3 grid = parts == 1 ? dim3(1, call.c.n_heads, call.b.n) : dim3((call.c.n_heads * call.b.n + 7) / 8 * 8 * parts);
+    const dim3 grid = parts == 1 ? dim3(1, call.c.n_heads, call.b.n) : dim3(workgroups(call, parts));
     const dim3 join(rows, call.c.n_heads, call.b.n);
     with_type(call.c, [&](auto t, auto d) {
         using T = decltype(t);
@@ -1163,8 +1177,8 @@ void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, const 
             using O = decltype(o);
             if (plan.many) {
                 constexpr int MW = 4;
-                const int tiles = plan.tiles / (MW * MR), groups = (call.c.n_heads * call.b.n + 7) / 8 * 8;
-                OWK_LAUNCH((k_kv8_attend_tiles<T, D, O, MW>), dim3(groups * tiles * plan.splits), dim3(MW * 64), 0, s, call, a, tiles);
+                const int tiles = plan.tiles / (MW * MR);
+                OWK_LAUNCH((k_kv8_attend_tiles<T, D, O, MW>), dim3(workgroups(call, tiles * plan.splits)), dim3(MW * 64), 0, s, call, a, tiles);
             } else if (plan.wide) {
                 if (plan.tiles == 1) OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 8, true>), grid, dim3(512), 0, s, call, a);
                 else OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 8, false>), grid, dim3(512), 0, s, call, a);

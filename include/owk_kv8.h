@@ -84,7 +84,7 @@ WHISPER_API int owk_kv8_append(const struct owk_kv8_cache * cache, const struct 
 
 struct owk_kv8_attend_params {
     int n_q_heads;  /* a multiple of n_heads; query head h reads key/value head h / (n_q_heads / n_heads) */
-    int causal;     /* 0: every row sees tokens [0, lens[b]), which are what the sequence holds;
+    int causal;     /* 0: every row sees tokens [0, lens[b]), which are what the sequence holds (or a multiple of 64 below);
                        1: row i sees [0, lens[b] + i], the call's own tokens were appended before */
     int out_type;   /* type of out: the cache's, or OWK_KV8_F32 */
     int max_len;    /* no sequence holds more tokens than this (decides how the work is split; 0: the capacity) */
@@ -112,6 +112,8 @@ WHISPER_API int owk_kv8_read(const struct owk_kv8_cache * cache, int n, int max_
 WHISPER_API void owk_debug_kv8_entry(const struct owk_kv8_cache * cache, const struct owk_kv8_batch * batch, int b,
                                      int64_t out[4]);
 WHISPER_API int64_t owk_debug_kv8_page(const struct owk_kv8_cache * cache, int seq, int i);
+/* test hook: owk_kv8_attend takes its many-row form for calls of more than `rows` rows a key/value head (0: by its own rule) */
+WHISPER_API void owk_debug_kv8_set_many_rows(int rows);
 
 /* what the calling thread's last failed call found wrong ("" if none failed) */
 WHISPER_API const char * owk_kv8_error(void);

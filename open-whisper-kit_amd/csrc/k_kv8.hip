@@ -5,7 +5,9 @@
 // operand that its matrix product reads along its sum (keys along D, values along the tokens), 16
 // contiguous bytes a lane. The incomplete last block (tail) lies in 16 bits in the same two orders.
 #include <algorithm>
+#include <atomic>
 #include <climits>
+#include <cmath>
 
 #include "kv8.h"
 
@@ -656,9 +658,12 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
 // keys 16 g .. 16 g + 15, and chunk k of eight of them is what O^T = V^T P^T wants as its k-th operand.
 // Probabilities are p = exp2(s - m) times 2^6 sv / sigma, sv the block's scale of values, sigma a power of two above it: the
 // accumulator is in units of sigma 2^-6 and the block's scale costs nothing. sigma moves (and the accumulator with it, an
-// exact step) when a scale is larger, or 2^-20 smaller and so near the end of half precision. m is brought up to
+// exact step) when a scale is larger, or so much smaller, 2^-8, that probabilities would lose bits at the end of half precision.
+// It stays within 2^-72 of the largest scale, so that the accumulator cannot overflow; a block further below (bf16 alone has
+// such) is added by f32 multiply-adds. m is brought up to
 // the running maximum only when a block's sum of them passes 2^14: they stay in range, and the accumulator is rarely rescaled.
-constexpr int MR = 2;  // row tiles of a wave
+constexpr int MR = 2;          // row tiles of a wave
+constexpr int MANY_WAVES = 4;  // of a workgroup
 
 // sixteen codes as half-precision floats: 0x6400 | x is 1024 + x
 __device__ __forceinline__ void to_half(const i32x4 & c, half8 (&h)[2]) {
@@ -899,7 +904,7 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
     float m[MR], l[MR];  // the same in all four lanes of a row
     floatx4 o[MR][DT];
-    int sig = INT_MIN;  // sigma = 2^sig
+    int sig = INT_MIN, peak = INT_MIN;  // sigma = 2^sig, and the largest it was
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
         m[r] = -INFINITY;
@@ -922,13 +927,14 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         ask(blk + 1);
         if (mine > base) {
             const bool part = !(there && whole && least >= base + BLK);  // some row does not see all of it
-            // sigma goes up with a larger scale, and down where a scale would come too near the end of half precision
             const int up = csv > 0.0f && finite(csv) ? ilogbf(csv) + 1 : INT_MIN;
             const int old = sig;
-            if (up != INT_MIN && (up > sig || up < sig - 20)) sig = old == INT_MIN ? up : max(up, old - 90);
+            peak = max(peak, up);
+            if (up != INT_MIN && (up > sig || up < sig - 8)) sig = max(up, peak - 72);
+            const bool far = up != INT_MIN && up < sig - 8;
             const float moved = old == INT_MIN ? 1.0f : ldexpf(1.0f, old - sig);
             // what a probability is multiplied by, and what its sum is divided by
-            const float mul = up == INT_MIN ? 64.0f : ldexpf(csv, 6 - sig);
+            const float mul = up == INT_MIN || far ? 64.0f : ldexpf(csv, 6 - sig);
             const float lg = csv == csv ? __builtin_amdgcn_logf(mul) : NAN, inv = csv == csv ? 1.0f / mul : NAN;
             uint32_t ph[MR][8];  // pairs of probabilities: of keys 16 g + 2 j, + 1
             int here[MR];
@@ -1014,6 +1020,23 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
                 for (int r = 0; r < MR; ++r)
                     if (max_over_g((int) (cbad & ((1u << min(max(here[r] - 16 * g, 0), 16)) - 1)))) l[r] = NAN;
             }
+            if (far) {
+                const float fo = ldexpf(csv, -sig);
+#pragma unroll
+                for (int r = 0; r < MR; ++r) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        floatx4 x = {0, 0, 0, 0};
+                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.v[mv[0] + d * 16 * (BLK / 8)], *(const half8 *) &ph[r][0], x, 0, 0, 0);
+                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.v[mv[1] + d * 16 * (BLK / 8)], *(const half8 *) &ph[r][4], x, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[r][d][i] = fmaf(x[i], fo, o[r][d][i]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) ph[r][j] = 0;
+                }
+            }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const half8 v0 = s.v[mv[0] + d * 16 * (BLK / 8)], v1 = s.v[mv[1] + d * 16 * (BLK / 8)];
@@ -1067,6 +1090,14 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     }
 }
 
+// splits that a tile of 16 rows has: those of the workgroup that made it
+__device__ __forceinline__ int splits_of(const Kv8Call & a, const Kv8Attend & p, const Kv8Entry & e, int tile) {
+    const int stored = e.seq < 0 ? 0 : p.causal ? min(e.start + e.n, a.c.max_blocks * BLK) : e.start;
+    const int last = min((tile / p.join + 1) * p.join * 16 - 1, e.n * p.group - 1) / p.group;
+    const int most = p.causal ? min(stored, e.start + last + 1) : stored;
+    return min(p.splits, max(1, ((most + BLK - 1) / BLK + p.per - 1) / p.per));
+}
+
 // joins the splits of a row, in order: a workgroup a row, its waves take every fourth split and are joined at the end
 template <int D, typename O> __global__ __launch_bounds__(256) void k_kv8_attend_join(Kv8Call a, Kv8Attend p) {
     constexpr int DL = D / 64;
@@ -1074,10 +1105,7 @@ template <int D, typename O> __global__ __launch_bounds__(256) void k_kv8_attend
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const Kv8Entry e = kv8_entry(a, b);
     if (r >= e.n * p.group) return;
-    const int stored = e.seq < 0 ? 0 : p.causal ? min(e.start + e.n, a.c.max_blocks * BLK) : e.start;
-    const int last = min((tile / p.join + 1) * p.join * 16 - 1, e.n * p.group - 1) / p.group;
-    const int most = p.causal ? min(stored, e.start + last + 1) : stored;
-    const int n = min(p.splits, max(1, ((most + BLK - 1) / BLK + p.per - 1) / p.per));
+    const int n = splits_of(a, p, e, tile);
     const float * ws = p.ws + ((((int64_t) b * a.c.n_heads + head) * p.tiles + tile) * p.splits * 16 + row) * (D + 2);
     float m = -INFINITY, l = 0.0f, x[DL] = {};
 #pragma unroll 4
@@ -1111,6 +1139,36 @@ template <int D, typename O> __global__ __launch_bounds__(256) void k_kv8_attend
     ((O *) row_at(a, p.out, e, b, r / p.group, head * p.group + r % p.group, sizeof(O)))[d] = (O) (sum == 0.0f ? 0.0f : v / sum);
 }
 
+// the same for many rows of few splits: a wave a row, four after each other (a workgroup a row took 90 us for 72k rows of two
+// splits, most of it to start the workgroups)
+template <int D, typename O> __global__ __launch_bounds__(256) void k_kv8_attend_join_rows(Kv8Call a, Kv8Attend p) {
+    constexpr int DL = D / 64;
+    const int tile = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Kv8Entry e = kv8_entry(a, b);
+    if (tile * 16 >= e.n * p.group) return;
+    const int n = splits_of(a, p, e, tile);
+    const float * ws = p.ws + (((int64_t) b * a.c.n_heads + head) * p.tiles + tile) * p.splits * 16 * (D + 2);
+    for (int row = 4 * w; row < 4 * w + 4; ++row) {
+        const int r = tile * 16 + row;
+        if (r >= e.n * p.group) return;
+        float m = -INFINITY, l = 0.0f, x[DL] = {};
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const float * y = ws + (k * 16 + row) * (D + 2);
+            const float mk = y[0], lk = y[1], top = fmaxf(m, mk);
+            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top), f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - top);
+            m = top;
+            l = l * alpha + (lk == lk ? f * lk : NAN);
+#pragma unroll
+            for (int i = 0; i < DL; ++i) x[i] = x[i] * alpha + f * y[2 + i * 64 + lane];
+        }
+        O * out = (O *) row_at(a, p.out, e, b, r / p.group, head * p.group + r % p.group, sizeof(O));
+#pragma unroll
+        for (int i = 0; i < DL; ++i) out[i * 64 + lane] = (O) (l == 0.0f ? 0.0f : x[i] / l);
+    }
+}
+
 // blocks of a sequence that n consecutive tokens can touch
 int touched(int n) { return (n + BLK - 2) / BLK + 1; }
 
@@ -1140,25 +1198,46 @@ void kv8_read(hipStream_t s, const Kv8Call & call, const int32_t * first, const 
     });
 }
 
-// How a call is run. Up to 32 rows of an entry and head (a step, beams, grouped heads) go in tiles of 16, more in tiles of
-// 128. The keys are cut into parts of `per` blocks, a workgroup each. Entries may differ much in length, so parts are equal
-// in size and not in number: long entries have more of them.
+static std::atomic<int> g_many_rows{0};
+void kv8_set_many_rows(int rows) { g_many_rows = rows; }
+
+// How a call is run: host arithmetic on its sizes. The keys are cut into parts of `per` blocks, a workgroup each; entries may
+// differ much in length, so parts are equal in size and not in number: long entries have more of them.
 Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) {
-    const int64_t rows = (int64_t) call.b.max_new * group;
-    const int64_t blocks = std::max<int64_t>(1, (max_len + BLK - 1) / BLK);
+    const int64_t rows = (int64_t) call.b.max_new * group, tiles16 = (rows + 15) / 16;
+    const int64_t blocks = std::max<int64_t>(1, (max_len + BLK - 1) / BLK), pairs = (int64_t) call.c.n_heads * call.b.n;
     Kv8Plan plan;
-    plan.many = rows > 32;
-    plan.waves = 4;
-    const int mrows = plan.waves * MR * 16;
-    const int64_t tiles = plan.many ? (rows + mrows - 1) / mrows : (rows + 15) / 16;
-    const int64_t groups = tiles * call.c.n_heads * call.b.n;
+    // Many-row tiles where there is work for them, counted in 16 rows times a block: at heads of 64, 32 clips of 64 rows (61k)
+    // take 54 us either way, of 96 rows 77 us in tiles of 16 and 67 in tiles of 128, 4 clips of 300 rows (36k) 35 and 45;
+    // at heads of 128, 4 chunks of 80 rows over 4000 keys (10k) 39 and 35, of 132 rows 52 and 42.
+    plan.many = rows > 32 && (double) tiles16 * pairs * blocks >= (call.c.head_dim == 64 ? 56000 : 13000);
+    if (const int over = g_many_rows.load()) plan.many = rows > over;
+    const int mrows = MANY_WAVES * MR * 16;
+    const int64_t tiles = plan.many ? (rows + mrows - 1) / mrows : tiles16;
+    const int64_t groups = tiles * pairs;
     int64_t per = blocks;
-    // few rows: 256 parts fill the card; parts of more than 32 blocks leave it unevenly loaded where lengths differ
-    if (!plan.many && blocks > 32) per = std::min<int64_t>(32, std::max<int64_t>(8, (groups * blocks + 255) / 256));
-    if (plan.many && groups < 256 && blocks > 16) per = std::max<int64_t>(8, (groups * blocks + 511) / 512);
+    plan.fits = rows <= 1 << 22 && groups < 1 << 24;
+    if (!plan.fits) return plan;
+    if (!plan.many) {
+        // 256 parts fill the card; parts of more than 32 blocks leave it unevenly loaded where lengths differ (16 streams of
+        // 900 to 33000 tokens: parts of 24 to 40 blocks 103 us, of 16 125, of 65 and of 129 over 140)
+        if (blocks > 32) per = std::min<int64_t>(32, std::max<int64_t>(8, (int64_t) std::min(std::ceil((double) groups * blocks / 256), 32.0)));
+    } else {
+        // rounds of the card (two or three workgroups on each of its 256 units) times the blocks of a part, and three more
+        // to begin and end it; joining costs some, too
+        const int64_t slots = call.c.head_dim == 64 ? 768 : 512;
+        int64_t best = INT64_MAX;
+        for (int64_t s = 1; s <= 8 && blocks >= 8 * s; ++s) {
+            const int64_t part = (blocks + s - 1) / s, cost = (groups * s + slots - 1) / slots * (part + 3) + (s > 1 ? 2 + groups / 100 : 0);
+            if (cost < best) best = cost, per = part;
+        }
+    }
     plan.splits = (int) ((blocks + per - 1) / per);
+    plan.fits = groups * plan.splits < (1 << 24) - 64;  // a one-dimensional grid: under 2^32 threads
+    if (!plan.fits) return plan;
     plan.per = (int) ((blocks + plan.splits - 1) / plan.splits);
     plan.tiles = (int) (plan.many ? tiles * (mrows / 16) : tiles);
+    plan.join = plan.many ? MANY_WAVES * MR : 1;
     plan.ws_bytes = plan.splits > 1 ? (size_t) plan.tiles * call.c.n_heads * call.b.n * plan.splits * 16 * (call.c.head_dim + 2) * 4 : 0;
     // few workgroups: eight waves rather than four share a tile's blocks
     plan.wide = !plan.many && plan.splits == 1 && groups <= 256;
@@ -1176,7 +1255,7 @@ void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, const 
         auto run = [&](auto o) {
             using O = decltype(o);
             if (plan.many) {
-                constexpr int MW = 4;
+                constexpr int MW = MANY_WAVES;
                 const int tiles = plan.tiles / (MW * MR);
                 OWK_LAUNCH((k_kv8_attend_tiles<T, D, O, MW>), dim3(workgroups(call, tiles * plan.splits)), dim3(MW * 64), 0, s, call, a, tiles);
             } else if (plan.wide) {
@@ -1186,7 +1265,10 @@ void kv8_attend(hipStream_t s, const Kv8Call & call, const Kv8Attend & a, const 
                 if (plan.tiles == 1) OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 4, true>), grid, dim3(256), 0, s, call, a);
                 else OWK_LAUNCH((k_kv8_attend_rows<T, D, O, 4, false>), grid, dim3(256), 0, s, call, a);
             }
-            if (plan.splits > 1) OWK_LAUNCH((k_kv8_attend_join<D, O>), join, dim3(256), 0, s, call, a);
+            if (plan.splits > 1 && plan.splits < 16 && rows >= 16)
+                OWK_LAUNCH((k_kv8_attend_join_rows<D, O>), dim3(plan.tiles, call.c.n_heads, call.b.n), dim3(256), 0, s, call, a);
+            else if (plan.splits > 1)
+                OWK_LAUNCH((k_kv8_attend_join<D, O>), join, dim3(256), 0, s, call, a);
         };
         if (out_type == OWK_KV8_F32) run(0.0f);
         else run(t);

@@ -128,6 +128,8 @@ void owk_debug_kv8_entry(const owk_kv8_cache * cache, const owk_kv8_batch * batc
     out[3] = e.row0;
 }
 
+void owk_debug_kv8_set_many_rows(int rows) { kv8_set_many_rows(rows); }
+
 int64_t owk_debug_kv8_page(const owk_kv8_cache * cache, int seq, int i) { return kv8_page(*cache, seq, i); }
 
 int owk_kv8_append(const owk_kv8_cache * cache, const owk_kv8_batch * batch, const owk_kv8_rows * k, const owk_kv8_rows * v,
@@ -157,6 +159,9 @@ int owk_kv8_attend(const owk_kv8_cache * cache, const owk_kv8_batch * batch, con
     if (int rc = check_rows("q", q, 2, a.q)) return rc;
     if (int rc = check_rows("out", out, params->out_type == OWK_KV8_F32 ? 4 : 2, a.out)) return rc;
     const Kv8Plan plan = plan_of(cache, batch, params);
+    if (!plan.fits)
+        return invalid("%d entries of up to %d rows and %d heads over up to %d tokens are too much for one call", batch->n, batch->max_new,
+                       params->n_q_heads, params->max_len > 0 ? params->max_len : capacity(cache));
     if (plan.ws_bytes > 0) {
         if (!workspace || workspace_bytes < plan.ws_bytes)
             return invalid("a workspace of %zu bytes is needed, %zu are there", plan.ws_bytes, workspace ? workspace_bytes : 0);
@@ -167,7 +172,7 @@ int owk_kv8_attend(const owk_kv8_cache * cache, const owk_kv8_batch * batch, con
     a.splits = plan.splits;
     a.per = plan.per;
     a.tiles = plan.tiles;
-    a.join = plan.many ? 2 * plan.waves : 1;
+    a.join = plan.join;
     a.scale = params->scale;
     a.ws = (float *) workspace;
     return on_device(cache->device,

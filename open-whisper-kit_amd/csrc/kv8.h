@@ -71,10 +71,13 @@ struct Kv8Attend {
 
 // the split and workspace of an attend call (host arithmetic on the call's sizes alone)
 struct Kv8Plan {
-    int splits, per, tiles, waves;
-    bool many, wide;
-    size_t ws_bytes;
+    int splits = 1, per = 0, tiles = 0;
+    int join = 1;              // tiles of 16 rows in a workgroup
+    bool many = false, wide = false;
+    bool fits = true;          // false: more rows or workgroups than a launch can have
+    size_t ws_bytes = 0;
 };
+void kv8_set_many_rows(int rows);  // for tests: calls of more rows a head run in many-row tiles; 0: by kv8_plan's own rule
 Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len);
 
 void kv8_append(hipStream_t s, const Kv8Call & call, const Kv8Rows & k, const Kv8Rows & v);

@@ -132,12 +132,26 @@ def assert_held(cache, model, lens):
             assert not got[x:].any()
 
 
-def check_attend(cache, model, lens, new, group, causal, layout="joined", out_type=None, scale=None, seed=3, width=1.0, max_len=0):
-    """Query rows new[b] for each sequence b; lens: tokens before the call's own."""
+def check_attend(cache, model, lens, new, group, causal, *args, **kw):
+    """Query rows new[b] for each sequence b; lens: tokens before the call's own. More than 32 rows a head can run in either
+    form, by how much work there is: both are checked, whichever this call would get."""
+    L = KV.load()
+    for rows in (32, 1 << 30) if max(new) * group > 32 else (0,):
+        cache._ws.clear()  # sizes of the other form's workspaces
+        L.owk_debug_kv8_set_many_rows(rows)
+        try:
+            _check_attend(cache, model, lens, new, group, causal, *args, **kw)
+        finally:
+            L.owk_debug_kv8_set_many_rows(0)
+            cache._ws.clear()
+
+
+def _check_attend(cache, model, lens, new, group, causal, layout="joined", out_type=None, scale=None, seed=3, width=1.0, max_len=0,
+                  rows=None):
     gen = torch.Generator().manual_seed(seed)
     hq, d, n = cache.n_heads * group, cache.head_dim, len(lens)
     scale = d ** -0.5 if scale is None else scale
-    rows = [normal(gen, x, hq, d, dtype=cache.dtype, width=width) for x in new]
+    rows = rows or [normal(gen, x, hq, d, dtype=cache.dtype, width=width) for x in new]
     out_type = out_type or cache.dtype
     mark = 7.25
     if layout == "joined":
@@ -269,6 +283,23 @@ def test_refused_workspaces():
     if need:  # one long sequence is cut into parts
         for ws, n in ((None, 0), (4096, need - 1), (4104, need)):
             assert L.owk_kv8_attend(d, b, _params(n_q_heads=1), _rows(), _rows(), ws, n, None) == -1
+
+
+@pytest.mark.parametrize("desc,batch,params", [
+    (dict(), dict(max_new=1 << 22), dict(n_q_heads=4)),                               # rows of a head
+    (dict(), dict(max_new=1 << 20), dict(n_q_heads=40000)),
+    (dict(n_heads=32000), dict(n=65535, max_new=1), dict(n_q_heads=32000)),           # tiles
+    (dict(n_heads=32000), dict(n=2000, max_new=1), dict(n_q_heads=32000)),
+    (dict(n_heads=2, n_seqs=1, n_blocks=1 << 24, max_blocks=1 << 24), dict(n=64, max_new=1), {}),  # parts of long sequences
+    (dict(n_heads=2, n_seqs=1, n_blocks=1 << 24, max_blocks=1 << 24), dict(n=65535, max_new=1 << 20), {}),
+])
+def test_refused_sizes(desc, batch, params):
+    """More workgroups than a launch can have."""
+    L = Raw()
+    d, b, p = _desc(**{"n_blocks": 1 << 20, **desc}), _batch(**batch), _params(**params)
+    assert L.owk_kv8_attend(d, b, p, _rows(), _rows(), 4096, 1 << 62, None) == -1
+    assert b"too much for one call" in KV.load().owk_kv8_error()
+    assert L.owk_kv8_attend_workspace(d, b, p) == 0
 
 
 def test_nothing_to_do_is_no_call():
@@ -521,6 +552,79 @@ def test_large_scores(dim, dtype):
     check_attend(cache, model, [333, 70], [2, 1], 1, False, width=4.0, scale=0.2)
     check_attend(cache, model, [333, 70], [64, 40], 1, False, width=4.0, scale=0.2)
     check_attend(cache, model, [333, 70], [2, 1], 1, False, width=4.0, scale=-0.2)
+
+
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("new", [2, 70])
+def test_blocks_of_different_size(dim, dtype, new):
+    """Values of a block 2^19 (bf16: up to 2^100) apart from the next one's, and rows that see little of the large ones:
+    what the small ones add keeps its bits."""
+    powers = [9, -10, -9, 0, -10, 3, 9, -12, -10] if dtype == F16 else [60, -20, -40, 3, -40, 40, 60, -30, -40]
+    n = 64 * len(powers) + 5
+    cache, model = make(1, 2, dim, n, dtype), Model(1, 2, dim, dtype)
+    gen = torch.Generator().manual_seed(12)
+    k, v = normal(gen, n, 2, dim, dtype=dtype, width=0.3), normal(gen, n, 2, dim, dtype=dtype)
+    size = torch.tensor(powers + powers[:1]).repeat_interleave(64)[:n, None, None].double()
+    v = (v.double() * 2.0 ** size).to(dtype)
+    k[:, :, 0] = torch.where(size[:, :, 0] > -9, -5.0, 5.0).to(dtype)  # the large ones: scores 100 below
+    cache.append(k[None].cuda(), v[None].cuda(), ints([0]))
+    model.append(0, 0, k, v)
+    q = normal(gen, new, 2, dim, dtype=dtype, width=0.3)
+    q[:, :, 0] = 10.0
+    q[1::2, :, 0] = 0.0  # every other row sees all of them alike
+    check_attend(cache, model, [n], [new], 1, False, rows=[q], scale=1.0)
+    check_attend(cache, model, [n - new], [new], 1, True, rows=[q], scale=1.0, out_type=torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16)])
+@pytest.mark.parametrize("new", [3, 20, 100])
+def test_joined_parts(dim, dtype, new):
+    """A few parts of the keys, for few rows and for many: joined a row at a time."""
+    lens, counts = [2500, 600, 2111, 64], [new, 1, new, new - 1]
+    held = [x + n for x, n in zip(lens, counts)]
+    cache, model = make(4, 1, dim, 2624, dtype, paged=True), Model(4, 1, dim, dtype)
+    fill(cache, model, held)
+    check_attend(cache, model, lens, counts, 1, True, layout="strided")
+    check_attend(cache, model, held, [1, new, 0, new], 2, False, out_type=torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("max_len", [1, 64, 700, 100000])
+@pytest.mark.parametrize("new", [1, 40])
+def test_lengths_beyond_the_hint(max_len, new):
+    """max_len only decides how the work is cut: sequences that hold more, or far less, come out right."""
+    lens = [1500, 0, 700, 63]
+    cache, model = make(4, 2, 64, 1600, F16), Model(4, 2, 64, F16)
+    fill(cache, model, lens)
+    check_attend(cache, model, lens, [new] * 4, 1, False, max_len=max_len)
+
+
+@gpu
+def test_entries_that_share_a_sequence():
+    """One sequence named by several entries of an attend call, at different lengths."""
+    cache, model = make(2, 2, 64, 400, F16), Model(2, 2, 64, F16)
+    fill(cache, model, [321, 130])
+    gen = torch.Generator().manual_seed(14)
+    seq, lens, new = [0, 1, 0, 0], [321, 130, 320 - 320 % 64, 64], 3
+    q = normal(gen, 4, new, 4, 64, dtype=F16)
+    got = cache.attend(q.cuda(), ints(lens), seq=ints(seq)).cpu().double()
+    for b in range(4):
+        want, bound = attend(q[b], model.held(seq[b], "k"), model.held(seq[b], "v"), 0.125, [lens[b]] * new, F16)
+        assert ((got[b] - want).abs() <= bound).all(), b
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_output_over_the_queries(new):
+    """A call may write where its queries are."""
+    cache, model = make(2, 2, 64, 200, F16), Model(2, 2, 64, F16)
+    fill(cache, model, [190, 65])
+    gen = torch.Generator().manual_seed(15)
+    q = normal(gen, 2, new, 4, 64, dtype=F16).cuda()
+    want = cache.attend(q, ints([190, 65]))
+    assert torch.equal(cache.attend(q, ints([190, 65]), out=q), want)
 
 
 @gpu

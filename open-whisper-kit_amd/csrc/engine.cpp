@@ -1092,6 +1092,7 @@ void Engine::launch_decode(const DecShape & sh) {
 // from row r0, the attention kernels take the pass's AttnRow entries r0.. (absolute q_row) and the
 // key-split soft_max workspace of those rows, so a row group's results equal the whole pass's.
 void Engine::fused_part(const DecShape & sh, int r0, int n, hipStream_t s, const GemmWs * ws) {
+    if (kv8_ && (r0 != 0 || n != sh.R)) throw std::runtime_error("decode: kv8 attention takes all rows of a pass");
     const HParams & hp = m->hp;
     const int d = hp.n_text_state, H = hp.n_text_head, T = n_ctx();
     const int n_ctx_pad = (T + 255) / 256 * 256;

@@ -178,7 +178,8 @@ class Cache:
     def attend(self, q, lens, seq=None, off=None, count=None, max_new=None, max_len=0, scale=None, causal=False, out=None):
         """softmax(scale * q . k) . v over what the sequences hold: tokens [0, lens[b]), or with causal, for row i,
         [0, lens[b] + i] (its own tokens appended before). scale None: 1 / sqrt(head_dim). `max_len`: no sequence holds
-        more (a hint for splitting the work). `out`: a tensor like q, or float32; rows that are no entry's stay as they are."""
+        more (a hint for splitting the work). `out`: a tensor like q, or float32; rows that are no entry's stay as they are (undefined in a new
+        tensor). No gradients."""
         shape = q.shape
         b, n, max_new = self._batch(shape, lens, seq, off, count, max_new)
         heads = shape[-2]

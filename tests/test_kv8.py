@@ -770,6 +770,35 @@ def test_captured_step(long):
 
 
 @gpu
+@pytest.mark.parametrize("many", [32, 1 << 30])
+def test_captured_chunk(many):
+    """A chunk of many rows over parts of the keys, captured once; each replay, with other lengths, equals the eager call."""
+    n, new, cap = 2, 40, 2240
+    cache = make(n, 2, 128, cap, BF16, paged=True)
+    gen = torch.Generator().manual_seed(16)
+    k, v = (normal(gen, n, cap, 2, 128, dtype=BF16).cuda() for _ in "kv")
+    cache.append(k, v, ints([0] * n))
+    q = normal(gen, n, new, 4, 128, dtype=BF16).cuda()
+    lens = ints([0, 0])
+    L = KV.load()
+    L.owk_debug_kv8_set_many_rows(many)
+    try:
+        cache.attend(q, lens)  # the workspace's size
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = cache.attend(q, lens)
+        for at in ([cap, 64], [0, 1280], [1920, 128], [640, cap], [64, 0]):  # whole blocks of what is held
+            lens.copy_(ints(at))
+            g.replay()
+            torch.cuda.synchronize()
+            want = cache.attend(q, lens)
+            assert want.isfinite().all() and torch.equal(out, want), at
+            assert all((out[b] != 0).any() == (at[b] > 0) for b in range(n)), at
+    finally:
+        L.owk_debug_kv8_set_many_rows(0)
+
+
+@gpu
 def test_other_streams_and_repeats():
     """A call on a side stream, and the same call twice: the same bits."""
     cache, model = make(4, 2, 64, 3000, F16), Model(4, 2, 64, F16)

@@ -960,7 +960,7 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         const Stage<D> & s = st[(blk - lo) & 1];
         const int base = blk * BLK;
         const bool there = held;
-        const float cks = ks, csv = sv;
+        const float cks = there ? ks : 0.0f, csv = there ? sv : 0.0f;  // (a block that is not there: its scales are block 0's)
         const uint32_t cbad = bad;
         ask(blk + 1);
         if (mine > base) {

@@ -1,0 +1,79 @@
+"""The 8-bit key/value cache at the edges of its types and tables: what a row sees of blocks of very different size, of
+hidden blocks, of values that are not finite, in both forms of attention (16-row and 128-row tiles). Oracle and bounds are
+test_kv8.py's."""
+import contextlib
+import math
+
+import pytest
+import torch
+
+import owk_kv8 as KV
+from test_kv8 import BF16, BLOCK, F16, Model, attend, check_attend, fill, ints, make, normal
+
+gpu = pytest.mark.gpu
+FORMS = [32, 1 << 30]  # rows of a head above which tiles of 128 rows are taken
+
+
+@contextlib.contextmanager
+def form(cache, rows):
+    L = KV.load()
+    cache._ws.clear()
+    L.owk_debug_kv8_set_many_rows(rows)
+    try:
+        yield
+    finally:
+        L.owk_debug_kv8_set_many_rows(0)
+        cache._ws.clear()
+
+
+def one_head(dtype, k, v, paged=False):
+    """A cache and model of one sequence that hold k, v [tokens, heads, dim] (given in 64 bits, rounded to dtype)."""
+    n, h, d = k.shape
+    cache, model = make(1, h, d, n, dtype, paged=paged), Model(1, h, d, dtype)
+    k, v = k.to(dtype), v.to(dtype)
+    cache.append(k[None].cuda(), v[None].cuda(), ints([0]))
+    model.append(0, 0, k, v)
+    return cache, model
+
+
+def spread(gen, *shape):
+    """Magnitudes in [1, 2), signs at random, in 64 bits."""
+    x = torch.rand(shape, generator=gen, dtype=torch.float64)
+    return (1 + x) * (2.0 * (torch.rand(shape, generator=gen) < 0.5) - 1)
+
+
+# ---------------------------------------------------------------------------------------------------
+# hidden blocks
+# ---------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("rows", FORMS)
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (64, BF16), (128, BF16)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_nothing_is_seen_of_a_hidden_block(dim, dtype, rows, causal):
+    """Whatever the pool's blocks hold, a table entry out of the pool adds nothing: the same bits."""
+    n, new, h = 3 * BLOCK + 7, 40, 2
+    gen = torch.Generator().manual_seed(31)
+    table = torch.tensor([[3, 1, 2, 4]], dtype=torch.int32, device="cuda")  # block 0 of the pool is no sequence's
+    cache, model = KV.Cache(1, h, dim, 256, dtype, "cuda", n_blocks=6, table=table), Model(1, h, dim, dtype)
+    k, v = (normal(gen, n, h, dim, dtype=dtype) for _ in "kv")
+    if dtype == BF16:
+        v = (v.double() * 2.0 ** -60).to(dtype)
+    cache.append(k[None].cuda(), v[None].cuda(), ints([0]))
+    model.append(0, 0, k, v)
+    table[0, 1] = -1
+    q = normal(gen, 1, new, h, dim, dtype=dtype).cuda()
+    at = n - new if causal else n
+    cache.k[0], cache.v[0] = 77, -33
+    outs = []
+    with form(cache, rows):
+        for scale in (0.0, 1.0, 2.0 ** 100, math.inf, math.nan):
+            cache.k_scale[0], cache.v_scale[0] = scale, scale
+            outs.append(cache.attend(q, ints([at]), causal=causal, out=torch.zeros_like(q, dtype=torch.float32)))
+    for x in outs[1:]:
+        assert torch.equal(x, outs[0])
+    keep = torch.cat([torch.arange(0, 64), torch.arange(128, n)])
+    kk, vv = model.held(0, "k")[keep], model.held(0, "v")[keep]
+    seen = [int((keep <= at + i).sum()) if causal else keep.numel() for i in range(new)]
+    want, bound = attend(q[0].cpu(), kk, vv, dim ** -0.5, seen, torch.float32)
+    # (the bound's blocks of 64 start at other tokens than the cache's, with at most twice the spread of probabilities)
+    assert ((outs[0][0].cpu().double() - want).abs() <= 2 * bound).all()

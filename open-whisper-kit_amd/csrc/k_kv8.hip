@@ -331,9 +331,10 @@ template <int D> struct Acc {
     }
 };
 
-// the tail of a sequence: the same tile on 16x16x32 products of the tail's own 16-bit type, with f32 sums. Half-precision
-// probabilities are held times 2^14 (small ones stay normal), bf16 ones as a sum of two. A token whose values are not all
-// finite makes the rows that see it NaN and touches no other.
+// the tail of a sequence, in both forms of attention: the same tile on 16x16x32 products of the tail's own 16-bit type, with f32
+// sums, so that a token's size is nothing to the others. Half-precision probabilities are held times 2^14 (small ones stay
+// normal), bf16 ones as a sum of two. A token whose values are not all finite makes the rows that see it NaN and touches no
+// other; a key that is not finite does unless its score is -inf, which has no weight.
 __device__ __forceinline__ floatx4 mfma16(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -747,8 +748,6 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     constexpr int DT = D / 16, KC = D / 32, NC = BLK * D / 16 / NT;  // NC: 16-byte pieces of codes of a thread
     constexpr bool BF = !std::is_same<T, _Float16>::value;
     __shared__ __align__(16) Stage<D> st[2];
-    __shared__ float red[2][MW];
-    __shared__ unsigned long long odd_keys;
     const Place place = place_of(a, tiles * p.splits);
     if (place.group < 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
@@ -817,7 +816,6 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         entry_n = blk < codes ? a.c.table ? a.c.table[(int64_t) e.seq * a.c.max_blocks + blk + zero] : e.seq * a.c.max_blocks + blk : -1;
     };
     ask_entry(lo);
-    uint32_t bad = 0;   // tokens of the lane's 16 that are not finite (tail)
     auto ask = [&](int blk) {
         const int page = __builtin_amdgcn_readfirstlane(entry_n);
         nheld = page >= 0 && page < a.c.n_blocks;
@@ -855,76 +853,6 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         ks = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(nks)));
         sv = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(nsv)));
     };
-    // the tail, from its 16-bit values; bf16 is brought into the range of f16 by a power of two, as queries are
-    auto put_tail = [&](Stage<D> & s) {
-        const int have = stored - full * BLK;
-        const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
-        const T * kt = (const T *) a.c.k_tail + t;
-        const T * vt = (const T *) a.c.v_tail + t;
-        if (threadIdx.x == 0) odd_keys = 0;
-        __syncthreads();
-        float tk = 0.0f, tv = 0.0f;
-        unsigned long long odd = 0;
-        for (int n = threadIdx.x; n < BLK * D / 8; n += NT) {
-            T x[8];
-            load_row<T, 8>(kt + n * 8, true, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (n / (D / 8) < have && finite(to_f32(x[i]))) tk = fmaxf(tk, fabsf(to_f32(x[i])));
-            load_row<T, 8>(vt + n * 8, true, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int key = n % (BLK / 8) * 8 + i;
-                const float y = fabsf(to_f32(x[i]));
-                if (key < have) {
-                    if (finite(y)) tv = fmaxf(tv, y);
-                    else odd |= 1ull << key;
-                }
-            }
-        }
-        if (odd) atomicOr(&odd_keys, odd);  // (bits: their order does not matter)
-        tk = wave_max(tk);
-        tv = wave_max(tv);
-        if (lane == 0) {
-            red[0][w] = tk;
-            red[1][w] = tv;
-        }
-        __syncthreads();
-        int ek = 0, ev = 0;
-        if (BF) {
-#pragma unroll
-            for (int i = 0; i < MW; ++i) {
-                tk = fmaxf(tk, red[0][i]);
-                tv = fmaxf(tv, red[1][i]);
-            }
-            ek = tk > 0.0f ? ilogbf(tk) : 0;
-            ev = tv > 0.0f ? ilogbf(tv) : 0;
-        }
-        for (int n = threadIdx.x; n < BLK * D / 8; n += NT) {
-            T x[8];
-            half8 h;
-            load_row<T, 8>(kt + n * 8, true, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = n / (D / 8) < have ? to_f32(x[i]) : 0.0f;
-                h[i] = (_Float16) (BF ? ldexpf(y, -ek) : y);
-            }
-            s.k[Stage<D>::at_k(n / (D / 8), n % (D / 8))] = h;
-            load_row<T, 8>(vt + n * 8, true, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float y = to_f32(x[i]);
-                if (n % (BLK / 8) * 8 + i >= have || !finite(y)) y = 0.0f;
-                h[i] = (_Float16) (BF ? ldexpf(y, -ev) : y);
-            }
-            s.v[Stage<D>::at_v(n / (BLK / 8), n % (BLK / 8))] = h;
-        }
-        held = true;
-        ks = ldexpf(1.0f, ek);
-        sv = ldexpf(1.0f, ev);
-        bad = (uint32_t) (odd_keys >> 16 * g) & 0xffff;
-    };
-
     // the scores of a staged block, in units of the block's and the rows' scales
     auto scores = [&](const Stage<D> & s, floatx4 (&x)[MR][4]) {
 #pragma unroll
@@ -954,14 +882,12 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
 
     ask(lo);
     if (lo < codes) put(st[0]);
-    else if (lo < hi) put_tail(st[0]);
     __syncthreads();
-    for (int blk = lo; blk < hi; ++blk) {
+    for (int blk = lo; blk < codes; ++blk) {
         const Stage<D> & s = st[(blk - lo) & 1];
         const int base = blk * BLK;
         const bool there = held;
         const float cks = there ? ks : 0.0f, csv = there ? sv : 0.0f;  // (a block that is not there: its scales are block 0's)
-        const uint32_t cbad = bad;
         ask(blk + 1);
         if (mine > base) {
             const bool part = !(there && whole && least >= base + BLK);  // some row does not see all of it
@@ -1056,11 +982,6 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
 #pragma unroll
             for (int r = 0; r < MR; ++r)
                 if (here[r] > 0) l[r] = fmaf(sum[r][0], inv, l[r]);
-            if (__any(cbad != 0)) {
-#pragma unroll
-                for (int r = 0; r < MR; ++r)
-                    if (max_over_g((int) (cbad & ((1u << min(max(here[r] - 16 * g, 0), 16)) - 1)))) l[r] = NAN;
-            }
             if (far) {
                 const float fo = ldexpf(csv, -sig);
 #pragma unroll
@@ -1091,37 +1012,50 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
             __builtin_amdgcn_s_setprio(0);
         }
         if (blk + 1 < codes) put(st[(blk + 1 - lo) & 1]);
-        else if (blk + 1 < hi) put_tail(st[(blk + 1 - lo) & 1]);
         __syncthreads();
     }
 
     // lane (c, g) holds dimensions 16 d + 4 g .. + 3 of its rows
     const float fin = sig == INT_MIN ? 0.0f : ldexpf(1.0f, sig - 6);
+    const bool tail = hi > full && mine > full * BLK;
+    const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
         const int row = row0 + r * 16 + c;
-        const float sum = l[r];
+        Acc<D> acc;
+        acc.m = m[r];
+        acc.l = 0.25f * l[r];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc.o[d][i] = o[r][d][i] * fin;
+        if (tail && row0 + r * 16 < nrows) {
+            const T * qr = row < nrows ? (const T *) row_at(a, p.q, e, b, row / p.group, head * p.group + row % p.group, 2) : nullptr;
+            attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qr, p.q.vec, p.scale * LOG2E, stored - full * BLK,
+                              see[r] - full * BLK, acc);
+        }
+        const float sum = sum_over_g(acc.l);
         if (row >= nrows) continue;
         if (p.splits > 1) {
             const int64_t t16 = (int64_t) tiles * (MROWS / 16);
             float * ws = p.ws + (((((int64_t) b * a.c.n_heads + head) * t16 + row / 16) * p.splits + split) * 16 + row % 16) * (D + 2);
             if (g == 0) {
-                ws[0] = m[r];
+                ws[0] = acc.m;
                 ws[1] = sum;
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) ws[2 + d * 16 + 4 * g + i] = o[r][d][i] * fin;
+                for (int i = 0; i < 4; ++i) ws[2 + d * 16 + 4 * g + i] = acc.o[d][i];
         } else {
             O * out = (O *) row_at(a, p.out, e, b, row / p.group, head * p.group + row % p.group, sizeof(O));
-            const float f = sum == 0.0f ? 0.0f : fin / sum;
+            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 typedef O vec4 __attribute__((ext_vector_type(4)));
                 vec4 y;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = (O) (sum == 0.0f ? 0.0f : o[r][d][i] * f);
+                for (int i = 0; i < 4; ++i) y[i] = (O) (sum == 0.0f ? 0.0f : acc.o[d][i] * f);
                 if (p.out.vec) {
                     *(vec4 *) (out + d * 16 + 4 * g) = y;
                 } else {

@@ -77,3 +77,36 @@ def test_nothing_is_seen_of_a_hidden_block(dim, dtype, rows, causal):
     want, bound = attend(q[0].cpu(), kk, vv, dim ** -0.5, seen, torch.float32)
     # (the bound's blocks of 64 start at other tokens than the cache's, with at most twice the spread of probabilities)
     assert ((outs[0][0].cpu().double() - want).abs() <= 2 * bound).all()
+
+
+# ---------------------------------------------------------------------------------------------------
+# tails
+# ---------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("before", [0, 64])
+def test_later_tokens_of_the_tail(dim, before):
+    """Causal rows over a bf16 tail: the size of later tokens' keys and values is nothing to a row."""
+    gen = torch.Generator().manual_seed(43)
+    new = 40
+    n = before + new
+    v, k = spread(gen, n, 1, dim), 0.3 * spread(gen, n, 1, dim)
+    v[before + 20:] *= 2.0 ** 40
+    k[before + 30:] *= 2.0 ** 60
+    cache, model = one_head(BF16, k, v)
+    check_attend(cache, model, [before], [new], 1, True, scale=1.0, out_type=torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_large_key_of_the_tail(dim):
+    """A key of the tail that no row attends to, far larger than the others."""
+    gen = torch.Generator().manual_seed(44)
+    n, new = 50, 40
+    v, k = spread(gen, n, 1, dim), 0.3 * spread(gen, n, 1, dim)
+    k[5, :, 0] = -2.0 ** 23  # (the bound stays finite)
+    v[5] = 2.0 ** 40
+    cache, model = one_head(BF16, k, v)
+    q = 0.3 * torch.randn((new, 1, dim), generator=gen)
+    q[:, :, 0] = 1.0
+    check_attend(cache, model, [n], [new], 1, False, rows=[q.to(BF16)], scale=1.0, out_type=torch.float32)

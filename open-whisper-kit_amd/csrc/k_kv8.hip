@@ -641,8 +641,8 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
 
     if (blk == full && blk < hi) {
         const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
-        attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qrow, p.q.vec, p.scale * LOG2E, stored - full * BLK,
-                          see - full * BLK, acc);
+        attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qrow, p.q.vec, qunit == qunit ? p.scale * LOG2E : NAN,
+                          stored - full * BLK, see - full * BLK, acc);
     }
 
     // join the waves, in order
@@ -778,28 +778,30 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         const T * qr = row < nrows ? (const T *) row_at(a, p.q, e, b, row / p.group, head * p.group + row % p.group, 2) : nullptr;
         T x[KC][8];
         float top = 0.0f;
+        bool ok = true;
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
             if (qr) load_row<T, 8>(qr + k * 32 + g * 8, p.q.vec, x[k]);
             else
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[k][i] = (T) 0.0f;
-            if (BF)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, finite(to_f32(x[k][i])) ? fabsf(to_f32(x[k][i])) : 0.0f);
+            for (int i = 0; i < 8; ++i) {
+                ok &= finite(to_f32(x[k][i]));
+                top = fmaxf(top, fabsf(to_f32(x[k][i])));
+            }
         }
+        // a row that is not finite has a unit that is NaN, and zeros for queries
+        top = max_over_g(ok ? top : INFINITY);
+        ok = finite(top);
         // bf16 rows are brought to [1, 2) by a power of two, exact but for what is 2^-14 of the largest or less
-        int ex = 0;
-        if (BF) {
-            top = max_over_g(top);
-            ex = top > 0.0f ? ilogbf(top) : 0;
-        }
-        unit[r] = ldexpf(fabsf(p.scale) * LOG2E, ex);
+        const int ex = BF && ok && top > 0.0f ? ilogbf(top) : 0;
+        unit[r] = ok ? ldexpf(fabsf(p.scale) * LOG2E, ex) : NAN;
         const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
         for (int k = 0; k < KC; ++k)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[r][k][i] = (_Float16) (BF ? ldexpf(to_f32(x[k][i]), -ex) * sgn : to_f32(x[k][i]) * sgn);
+            for (int i = 0; i < 8; ++i) q[r][k][i] = (_Float16) (!ok ? 0.0f : BF ? ldexpf(to_f32(x[k][i]), -ex) * sgn : to_f32(x[k][i]) * sgn);
     }
 
     // staging of block blk into s: its codes are asked for a block ahead, 16 of keys and of values a thread and piece
@@ -1031,8 +1033,8 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
             for (int i = 0; i < 4; ++i) acc.o[d][i] = o[r][d][i] * fin;
         if (tail && row0 + r * 16 < nrows) {
             const T * qr = row < nrows ? (const T *) row_at(a, p.q, e, b, row / p.group, head * p.group + row % p.group, 2) : nullptr;
-            attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qr, p.q.vec, p.scale * LOG2E, stored - full * BLK,
-                              see[r] - full * BLK, acc);
+            attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qr, p.q.vec, unit[r] == unit[r] ? p.scale * LOG2E : NAN,
+                              stored - full * BLK, see[r] - full * BLK, acc);
         }
         const float sum = sum_over_g(acc.l);
         if (row >= nrows) continue;

@@ -110,3 +110,30 @@ def test_one_large_key_of_the_tail(dim):
     q = 0.3 * torch.randn((new, 1, dim), generator=gen)
     q[:, :, 0] = 1.0
     check_attend(cache, model, [n], [new], 1, False, rows=[q.to(BF16)], scale=1.0, out_type=torch.float32)
+
+
+# ---------------------------------------------------------------------------------------------------
+# queries that are not finite
+# ---------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("rows", FORMS)
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, F16), (64, BF16), (128, BF16)])
+@pytest.mark.parametrize("n", [0, 20, 64, 100])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_queries_that_are_not_finite(dim, dtype, rows, n, bad):
+    """A row with such a query is NaN if it sees anything, and no other row is."""
+    gen = torch.Generator().manual_seed(46)
+    new = 40
+    k, v = spread(gen, max(n, 1), 1, dim), spread(gen, max(n, 1), 1, dim)
+    k[..., 3] = k[..., 3].abs()  # all scores of one sign
+    cache, _ = one_head(dtype, k, v)
+    q = normal(gen, 1, new, 1, dim, dtype=dtype).cuda()
+    for q_rows, count in ((q, new), (q[:, :3].contiguous(), 3)):
+        with form(cache, rows):
+            clean = cache.attend(q_rows, ints([n]))
+            x = q_rows.clone()
+            x[0, 1, 0, 3] = bad
+            got = cache.attend(x, ints([n]))
+        others = [i for i in range(count) if i != 1]
+        assert clean.isfinite().all() and got[0, others].isfinite().all()
+        assert got[0, 1].isnan().all() if n else not got[0, 1].any()

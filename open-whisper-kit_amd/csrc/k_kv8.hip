@@ -477,6 +477,7 @@ template <bool ONCE> __device__ __forceinline__ i32x4 load_codes(const int8_t * 
 template <typename T, int D, typename O, int W, bool ONCE>
 __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8Call a, Kv8Attend p) {
     constexpr int DT = D / 16, KC = D / 64;
+    constexpr bool BF = !std::is_same<T, _Float16>::value;
     int head = blockIdx.y, b = blockIdx.z, split = 0, tile = 0;
     if (gridDim.x > 1) {
         const Place place = place_of(a, p.tiles * p.splits);
@@ -544,6 +545,7 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
 
     i32x4 qh[KC], ql[KC];
     float qunit;
+    int qex = 0;
     {
         float top = 0.0f;
         bool ok = true;
@@ -556,12 +558,14 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
                 top = fmaxf(top, y);
             }
         top = max_over_g(ok ? top : INFINITY);
-        float inv = finite(top) && top > 0.0f ? UNIT / top : 0.0f;
-        // a row whose largest element is so small that UNIT / top overflows counts as zeros
-        qunit = finite(top) ? (finite(inv) ? top / UNIT : 0.0f) * fabsf(p.scale) * LOG2E : NAN;
-        inv = finite(inv) ? p.scale < 0.0f ? -inv : inv : 0.0f;
+        const bool any = finite(top) && top > 0.0f;
+        // a bf16 row is brought to [1, 2) by a power of two that goes to the blocks' scales: neither UNIT / top nor the unit
+        // leaves the range of f32 then, however small or large the queries are
+        if (BF && any) qex = ilogbf(top);
+        const float most = BF ? ldexpf(top, -qex) : top, inv = any ? p.scale < 0.0f ? -UNIT / most : UNIT / most : 0.0f;
+        qunit = finite(top) ? most / UNIT * fabsf(p.scale) * LOG2E : NAN;
         // what is not finite goes in as zero: the row's unit is NaN then
-        auto q = [&](int k, int i) { return ok ? to_f32(qx[k][i]) : 0.0f; };
+        auto q = [&](int k, int i) { return !ok ? 0.0f : BF ? ldexpf(to_f32(qx[k][i]), -qex) : to_f32(qx[k][i]); };
 #pragma unroll
         for (int k = 0; k < KC; ++k)
 #pragma unroll
@@ -575,7 +579,7 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
 
     Acc<D> acc;
     for (; blk < codes; blk += W) {
-        const float f = qunit * ks, svl = sv;
+        const float f = qunit * (BF ? ldexpf(ks, qex) : ks), svl = sv;
         const int here = held ? see - blk * BLK : 0;
         const bool all = held && least >= blk * BLK + BLK;  // every row of the tile sees the whole block
         int s[4][4], top = INT_MIN;
@@ -770,7 +774,7 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     // queries
     half8 q[MR][KC];
     float unit[MR];
-    int see[MR];
+    int see[MR], qex[MR];
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
         const int row = row0 + r * 16 + c;
@@ -795,13 +799,13 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         top = max_over_g(ok ? top : INFINITY);
         ok = finite(top);
         // bf16 rows are brought to [1, 2) by a power of two, exact but for what is 2^-14 of the largest or less
-        const int ex = BF && ok && top > 0.0f ? ilogbf(top) : 0;
-        unit[r] = ok ? ldexpf(fabsf(p.scale) * LOG2E, ex) : NAN;
+        qex[r] = BF && ok && top > 0.0f ? ilogbf(top) : 0;
+        unit[r] = ok ? fabsf(p.scale) * LOG2E : NAN;
         const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
         for (int k = 0; k < KC; ++k)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[r][k][i] = (_Float16) (!ok ? 0.0f : BF ? ldexpf(to_f32(x[k][i]), -ex) * sgn : to_f32(x[k][i]) * sgn);
+            for (int i = 0; i < 8; ++i) q[r][k][i] = (_Float16) (!ok ? 0.0f : BF ? ldexpf(to_f32(x[k][i]), -qex[r]) * sgn : to_f32(x[k][i]) * sgn);
     }
 
     // staging of block blk into s: its codes are asked for a block ahead, 16 of keys and of values a thread and piece
@@ -908,7 +912,7 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
 #pragma unroll
             for (int r = 0; r < MR; ++r) {
                 here[r] = part ? there ? see[r] - base : 0 : BLK;
-                f[r] = unit[r] * cks;
+                f[r] = unit[r] * (BF ? ldexpf(cks, qex[r]) : cks);
                 by[r] = moved;
             }
             // the probabilities by the m there is, and their sum by a product with ones (what is summed is what multiplies

@@ -137,3 +137,21 @@ def test_queries_that_are_not_finite(dim, dtype, rows, n, bad):
         others = [i for i in range(count) if i != 1]
         assert clean.isfinite().all() and got[0, others].isfinite().all()
         assert got[0, 1].isnan().all() if n else not got[0, 1].any()
+
+
+# ---------------------------------------------------------------------------------------------------
+# queries
+# ---------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("power,scale", [(-120, 0.125), (-110, 0.125), (110, 0.125), (126, 4.0), (126, -4.0)])
+@pytest.mark.parametrize("n", [64, 100, 150])
+def test_queries_of_any_size(dim, power, scale, n):
+    """Tiny queries of large keys and large queries of tiny keys: the same scores."""
+    gen = torch.Generator().manual_seed(45)
+    new = 40
+    k, v = 0.5 * spread(gen, n, 1, dim) * 2.0 ** -min(power, 118), spread(gen, n, 1, dim)
+    cache, model = one_head(BF16, k, v)
+    q = 0.5 * spread(gen, new, 1, dim) * 2.0 ** power
+    check_attend(cache, model, [n], [new], 1, False, rows=[q.to(BF16)], scale=scale, out_type=torch.float32)
+    check_attend(cache, model, [n], [2], 1, False, rows=[q[:2].to(BF16)], scale=scale, out_type=torch.float32)

@@ -696,12 +696,13 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
 //
 // The lanes hold what they hold above: S^T = K Q^T with the keys of a tile permuted so that lane (c, g) gets the scores of
 // keys 16 g .. 16 g + 15, and chunk k of eight of them is what O^T = V^T P^T wants as its k-th operand.
-// Probabilities are p = exp2(s - m) times 2^6 sv / sigma, sv the block's scale of values, sigma a power of two above it: the
-// accumulator is in units of sigma 2^-6 and the block's scale costs nothing. sigma moves (and the accumulator with it, an
-// exact step) when a scale is larger, or so much smaller, 2^-8, that probabilities would lose bits at the end of half precision.
-// It stays within 2^-72 of the largest scale, so that the accumulator cannot overflow; a block further below (bf16 alone has
-// such) is added by f32 multiply-adds. m is brought up to
-// the running maximum only when a block's sum of them passes 2^14: they stay in range, and the accumulator is rarely rescaled.
+// Probabilities are p = exp2(s - m) times 2^6 sv / 2^sig, sv the block's scale of values: the accumulator is in units of 2^(sig - 6)
+// and the block's scale costs nothing. m and sig are a row's own, and stay what they are as long as the block's sum of these
+// products lies in a window of half precision: at most 2^14, and at least what one product of 2^-10 makes, so that what is rounded
+// below the normal range is 2^-15 of the largest. A row that leaves the window makes its products again, with m brought up to the
+// running maximum and sig to what the block adds, p sv: values of any size under weights of any size keep their bits. sig
+// falls to 2^-64 of the largest it was at the most, so that the accumulator cannot overflow; what a block adds below that is
+// added by f32 multiply-adds. Rows are independent of each other: none sees another's m or sig.
 constexpr int MR = 2;          // row tiles of a wave
 constexpr int MANY_WAVES = 4;  // of a workgroup
 
@@ -876,11 +877,13 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
     float m[MR], l[MR];  // the same in all four lanes of a row
     floatx4 o[MR][DT];
-    int sig = INT_MIN, peak = INT_MIN;  // sigma = 2^sig, and the largest it was
+    constexpr float NONE = -0x1p20f;
+    float sig[MR], peak[MR];  // whole numbers; peak: the largest sig was, with what m moved up since taken off
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
         m[r] = -INFINITY;
         l[r] = 0.0f;
+        sig[r] = peak[r] = NONE;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[r][d] = floatx4{0, 0, 0, 0};
     }
@@ -897,30 +900,34 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         ask(blk + 1);
         if (mine > base) {
             const bool part = !(there && whole && least >= base + BLK);  // some row does not see all of it
-            const int up = csv > 0.0f && finite(csv) ? ilogbf(csv) + 1 : INT_MIN;
-            const int old = sig;
-            peak = max(peak, up);
-            if (up != INT_MIN && (up > sig || up < sig - 8)) sig = max(up, peak - 72);
-            const bool far = up != INT_MIN && up < sig - 8;
-            const float moved = old == INT_MIN ? 1.0f : ldexpf(1.0f, old - sig);
-            // what a probability is multiplied by, and what its sum is divided by
-            const float mul = up == INT_MIN || far ? 64.0f : ldexpf(csv, 6 - sig);
-            const float lg = csv == csv ? __builtin_amdgcn_logf(mul) : NAN, inv = csv == csv ? 1.0f / mul : NAN;
+            // the block's scale of values is svm 2^e2 (1 for a block of zeros, which adds to the sums alone)
+            const bool zero = csv == 0.0f;
+            const int e2 = __builtin_amdgcn_frexp_expf(csv);
+            const float svm = zero ? 1.0f : __builtin_amdgcn_frexp_mantf(csv);
+            const float inv = __builtin_amdgcn_rcpf(svm), lsv = __builtin_amdgcn_logf(svm);
+            const float low = zero ? 0.0f : 0x1p-10f;
             uint32_t ph[MR][8];  // pairs of probabilities: of keys 16 g + 2 j, + 1
-            int here[MR];
-            float f[MR], by[MR];  // by: what the accumulator is multiplied by
+            int here[MR], lag[MR];  // lag: the block's products are 2^lag above the accumulator's unit
+            float f[MR], by[MR], least_sum[MR];  // by: what the accumulator is multiplied by
+            float mm[MR], power[MR];  // p svm 2^power = exp2(s - mm)
 #pragma unroll
             for (int r = 0; r < MR; ++r) {
                 here[r] = part ? there ? see[r] - base : 0 : BLK;
                 f[r] = unit[r] * (BF ? ldexpf(cks, qex[r]) : cks);
-                by[r] = moved;
+                by[r] = 1.0f;
+                lag[r] = 0;
+                power[r] = zero ? 6.0f : (float) (e2 + 6) - sig[r];
+                mm[r] = m[r] - (power[r] + lsv);
+                // (no sum is large enough where p would be far above 1, or there is no sig yet)
+                least_sum[r] = ((power[r] >= -24.0f) & (power[r] < 4096.0f)) ? low * (float) (part ? min(here[r], BLK) : BLK) : INFINITY;
+                if (part) least_sum[r] = here[r] > 0 ? least_sum[r] : -INFINITY;
             }
-            // the probabilities by the m there is, and their sum by a product with ones (what is summed is what multiplies
-            // the values); where that is too large, or there is no m yet, m is brought up to the maximum and they are made again
+            // the products by the m and sig there are, and their sum by a product with ones (what is summed is what multiplies
+            // the values); rows that leave the window are made again
             floatx4 sum[MR];
 #pragma clang loop unroll(disable)
             for (int again = 0;; ++again) {
-                bool over = false;
+                bool out[MR];
                 floatx4 x[MR][4];
                 // (products before other waves' softmax: chunks 348 -> 333 us, prompts the same)
                 __builtin_amdgcn_s_setprio(1);
@@ -928,11 +935,10 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
                 __builtin_amdgcn_s_setprio(0);
 #pragma unroll
                 for (int r = 0; r < MR; ++r) {
-                    const float mm = (m[r] == -INFINITY ? 0.0f : m[r]) - lg;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float2v y = {__builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4], f[r], -mm)),
-                                           __builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4 + 1], f[r], -mm))};
+                        const float2v y = {__builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4], f[r], -mm[r])),
+                                           __builtin_amdgcn_exp2f(fmaf(x[r][j / 2][2 * j % 4 + 1], f[r], -mm[r]))};
                         ph[r][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, half2v));
                     }
                 }
@@ -952,8 +958,9 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
                     sum[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, *(const half8 *) &ph[r][4], sum[r], 0, 0, 0);
                 }
 #pragma unroll
-                for (int r = 0; r < MR; ++r) over |= sum[r][0] > 16384.0f || (m[r] == -INFINITY && here[r] > 0);
-                if (again || !__any(over)) break;
+                for (int r = 0; r < MR; ++r)
+                    out[r] = !((sum[r][0] <= 16384.0f) & (sum[r][0] >= least_sum[r]));
+                if (again || !__any(out[0] | out[MR - 1])) break;
 #pragma unroll
                 for (int r = 0; r < MR; ++r) {
                     float top = -INFINITY;
@@ -970,11 +977,27 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     top = max_over_g(top);
-                    const float mb = top == -INFINITY ? -INFINITY : top * f[r], next = fmaxf(m[r], mb);
-                    const float alpha = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - next);
-                    m[r] = next;
-                    l[r] *= alpha;
-                    by[r] *= alpha;
+                    if (out[r]) {
+                        const float mb = top == -INFINITY ? -INFINITY : top * f[r], next = fmaxf(m[r], mb);
+                        // m moves up by `steps` whole powers of two and a factor: the same in both products
+                        const float up = m[r] == -INFINITY ? 0.0f : next - m[r], steps = fminf(floorf(up), 1e5f);
+                        const float frac = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(steps - up);
+                        m[r] = next;
+                        l[r] *= ldexpf(frac, -(int) steps);
+                        float shift = -steps;
+                        if (sig[r] != NONE) peak[r] = fmaxf(peak[r] - steps, -1e5f);
+                        if (!zero && mb > -INFINITY) {
+                            const float own = (float) e2 + floorf(fmaxf(mb - next, -1e3f));  // of what the block adds
+                            peak[r] = fmaxf(peak[r], own);
+                            const float to = fmaxf(own, peak[r] - 64.0f);
+                            if (sig[r] != NONE) shift += sig[r] - to;
+                            sig[r] = to;
+                            lag[r] = (int) (to - own);
+                            power[r] = (float) (e2 + 6) - own;
+                        }
+                        by[r] = ldexpf(frac, (int) shift);
+                        mm[r] = (m[r] == -INFINITY ? 0.0f : m[r]) - (power[r] + lsv);
+                    }
                 }
             }
             if (__any(by[0] != 1.0f || by[MR - 1] != 1.0f)) {
@@ -987,22 +1010,26 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
             }
 #pragma unroll
             for (int r = 0; r < MR; ++r)
-                if (here[r] > 0) l[r] = fmaf(sum[r][0], inv, l[r]);
-            if (far) {
-                const float fo = ldexpf(csv, -sig);
+                if (here[r] > 0) l[r] = fmaf(sum[r][0], ldexpf(inv, -(int) power[r]), l[r]);
+            if (__any(lag[0] != 0 || lag[MR - 1] != 0)) {
 #pragma unroll
                 for (int r = 0; r < MR; ++r) {
+                    const float fo = ldexpf(1.0f, -lag[r]);
+                    uint32_t pf[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        pf[j] = lag[r] ? ph[r][j] : 0;
+                        ph[r][j] = lag[r] ? 0 : ph[r][j];
+                    }
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
                         floatx4 x = {0, 0, 0, 0};
-                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.v[mv[0] + d * 16 * (BLK / 8)], *(const half8 *) &ph[r][0], x, 0, 0, 0);
-                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.v[mv[1] + d * 16 * (BLK / 8)], *(const half8 *) &ph[r][4], x, 0, 0, 0);
+                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.v[mv[0] + d * 16 * (BLK / 8)], *(const half8 *) &pf[0], x, 0, 0, 0);
+                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.v[mv[1] + d * 16 * (BLK / 8)], *(const half8 *) &pf[4], x, 0, 0, 0);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[r][d][i] = fmaf(x[i], fo, o[r][d][i]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) ph[r][j] = 0;
                 }
             }
             __builtin_amdgcn_s_setprio(1);
@@ -1022,12 +1049,12 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     }
 
     // lane (c, g) holds dimensions 16 d + 4 g .. + 3 of its rows
-    const float fin = sig == INT_MIN ? 0.0f : ldexpf(1.0f, sig - 6);
     const bool tail = hi > full && mine > full * BLK;
     const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
         const int row = row0 + r * 16 + c;
+        const float fin = sig[r] == NONE ? 0.0f : ldexpf(1.0f, (int) sig[r] - 6);
         Acc<D> acc;
         acc.m = m[r];
         acc.l = 0.25f * l[r];

@@ -155,3 +155,78 @@ def test_queries_of_any_size(dim, power, scale, n):
     q = 0.5 * spread(gen, new, 1, dim) * 2.0 ** power
     check_attend(cache, model, [n], [new], 1, False, rows=[q.to(BF16)], scale=scale, out_type=torch.float32)
     check_attend(cache, model, [n], [2], 1, False, rows=[q[:2].to(BF16)], scale=scale, out_type=torch.float32)
+
+
+# ---------------------------------------------------------------------------------------------------
+# blocks of very different size
+# ---------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype,ratio", [(F16, 20), (F16, 24), (F16, 26), (F16, 28), (BF16, 30), (BF16, 45), (BF16, 60)])
+@pytest.mark.parametrize("order", ["small first", "large first", "in turn"])
+def test_large_values_of_small_weight(dim, dtype, ratio, order):
+    """A block whose values are 2^ratio larger and whose weights as much smaller adds as much as the others."""
+    gen = torch.Generator().manual_seed(ratio)
+    sizes = {"small first": [0, 1], "large first": [1, 0], "in turn": [0, 1, 0, 0, 1]}[order]
+    n, new = 64 * len(sizes) + 3, 40
+    big = torch.tensor(sizes + [0]).repeat_interleave(64)[:n, None, None]
+    v = spread(gen, n, 1, dim) * torch.where(big > 0, 2.0 ** (ratio // 2), 2.0 ** (ratio // 2 - ratio))
+    k = 0.2 * spread(gen, n, 1, dim)
+    k[:, :, 0] = torch.where(big[..., 0] > 0, -(ratio + 0.3) * math.log(2), 0.0)  # with q[0] = 1 and scale 1: the score's level
+    cache, model = one_head(dtype, k, v)
+    q = 0.3 * torch.randn((new, 1, dim), generator=gen)
+    q[:, :, 0] = 1.0
+    q[1::4, :, 0] = 1.25  # rows that see less and more of them
+    q[2::4, :, 0] = 0.75
+    check_attend(cache, model, [n], [new], 1, False, rows=[q.to(dtype)], scale=1.0, out_type=torch.float32)
+    check_attend(cache, model, [n - new], [new], 1, True, rows=[q.to(dtype)], scale=1.0, out_type=torch.float32)
+    check_attend(cache, model, [n], [2], 1, False, rows=[q[:2].to(dtype)], scale=1.0, out_type=torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_of_zero_under_a_large_weight(dim):
+    """One block takes nearly all of the weight and has values of zero: the rest is what the output is made of."""
+    gen = torch.Generator().manual_seed(41)
+    n, new = 4 * 64, 48
+    v, k = spread(gen, n, 1, dim), 0.2 * spread(gen, n, 1, dim)
+    k[:64, :, 0] = 24.0
+    v[:64] = 0.0
+    cache, model = one_head(BF16, k, v)
+    q = 0.3 * torch.randn((new, 1, dim), generator=gen)
+    q[:, :, 0] = 1.0
+    check_attend(cache, model, [n], [new], 1, False, rows=[q.to(BF16)], scale=1.0, out_type=torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("low,high", [(-40, 40), (-70, 80), (-100, 110)])
+def test_a_block_of_other_rows(dim, low, high):
+    """Causal rows of one tile: the size of a block that some of them see is nothing to those before it."""
+    gen = torch.Generator().manual_seed(42)
+    n, at = 3 * 64, 40
+    v, k = spread(gen, n, 1, dim), 0.3 * spread(gen, n, 1, dim)
+    v[:64] *= 2.0 ** low
+    v[64:128] *= 2.0 ** high
+    cache, model = one_head(BF16, k, v)
+    check_attend(cache, model, [at], [n - at], 1, True, scale=1.0, out_type=torch.float32)
+
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("rows", FORMS)
+def test_rows_do_not_depend_on_each_other(dim, dtype, rows):
+    """A row's bits are the same whatever the rows beside it are."""
+    gen = torch.Generator().manual_seed(53)
+    n, new = 300, 40
+    v, k = spread(gen, n, 1, dim), 0.5 * spread(gen, n, 1, dim)
+    v *= 2.0 ** torch.randint(-12, 12, (6, 1, 1), generator=gen).repeat_interleave(64, 0)[:n]
+    cache, _ = one_head(dtype, k, v)
+    q = 0.5 * spread(gen, 1, new, 1, dim)
+    with form(cache, rows):
+        want = cache.attend(q.to(dtype).cuda(), ints([n]), scale=1.0)
+        for other in (0.0, 12.0, math.nan):
+            x = q.clone()
+            x[:, ::3] *= other
+            got = cache.attend(x.to(dtype).cuda(), ints([n]), scale=1.0)
+            for i in (1, 2):
+                assert torch.equal(got[:, i::3], want[:, i::3]), (other, i)

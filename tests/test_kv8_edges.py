@@ -230,3 +230,124 @@ def test_rows_do_not_depend_on_each_other(dim, dtype, rows):
             got = cache.attend(x.to(dtype).cuda(), ints([n]), scale=1.0)
             for i in (1, 2):
                 assert torch.equal(got[:, i::3], want[:, i::3]), (other, i)
+
+
+# ---------------------------------------------------------------------------------------------------
+# keys and values that are not finite
+# ---------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, F16), (64, BF16), (128, BF16)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_a_complete_block_that_is_not_finite(dim, dtype, which, bad):
+    """It is NaN to the rows that see any of it: not to causal rows before it, nor to another head or sequence."""
+    lens = [230, 230]
+    cache, model = make(2, 2, dim, 320, dtype, paged=True), Model(2, 2, dim, dtype)
+    gen = torch.Generator().manual_seed(47)
+    for s, n in enumerate(lens):
+        k, v = (normal(gen, n, 2, dim, dtype=dtype) for _ in "kv")
+        if s == 0:
+            (k if which == "k" else v)[100, 1, 7] = bad
+        cache.append(k[None].cuda(), v[None].cuda(), ints([0]), seq=ints([s]))
+        model.append(s, 0, k, v)
+    check_attend(cache, model, lens, [40, 40], 1, False)
+    check_attend(cache, model, lens, [2, 2], 2, False)
+    check_attend(cache, model, [20, 20], [210, 210], 1, True)  # rows before it, in it and behind it
+    for at in (62, 63, 64, 127, 128):
+        check_attend(cache, model, [at, at], [lens[0] - at] * 2, 1, True, max_len=256)
+
+
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_parts_that_are_not_finite(dim, dtype, which, new):
+    """One part of a long sequence's keys is NaN: the join keeps it."""
+    lens = [6000, 6000]
+    cache, model = make(2, 1, dim, 6016, dtype, paged=True), Model(2, 1, dim, dtype)
+    gen = torch.Generator().manual_seed(48)
+    for s, n in enumerate(lens):
+        k, v = (normal(gen, n, 1, dim, dtype=dtype) for _ in "kv")
+        if s == 0:
+            (k if which == "k" else v)[4321, 0, 7] = math.nan
+        cache.append(k[None].cuda(), v[None].cuda(), ints([0]), seq=ints([s]))
+        model.append(s, 0, k, v)
+    check_attend(cache, model, lens, [new, new], 1, False)
+
+
+@gpu
+@pytest.mark.parametrize("rows", FORMS)
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, F16), (64, BF16), (128, BF16)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("before", [0, 64])
+def test_a_tail_token_that_is_not_finite(dim, dtype, rows, which, before):
+    """Only later causal rows see it, in its own head and sequence."""
+    new, odd = 50, before + 30
+    lens = [before, before]
+    cache, model = make(2, 2, dim, 128, dtype), Model(2, 2, dim, dtype)
+    fill(cache, model, [before + new] * 2)
+    gen = torch.Generator().manual_seed(49)
+    q = normal(gen, 2, new, 2, dim, dtype=dtype).cuda()
+    with form(cache, rows):
+        clean = cache.attend(q, ints(lens), causal=True)
+        if which == "k":
+            cache.k_tail[1, 0, odd % BLOCK, 5] = math.nan
+        else:
+            cache.v_tail[1, 0, 5, odd % BLOCK] = math.inf
+        got = cache.attend(q, ints(lens), causal=True)
+    sees = [lens[1] + i >= odd for i in range(new)]
+    assert clean.isfinite().all()
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1, :, 1], clean[1, :, 1])
+    for i in range(new):
+        if not sees[i]:
+            assert torch.equal(got[1, i, 0], clean[1, i, 0]), i
+        else:
+            assert not got[1, i, 0, 5].isfinite(), i
+            assert which == "v" or got[1, i, 0].isnan().all(), i
+
+
+# ---------------------------------------------------------------------------------------------------
+# the 128-row form in the calls that the 16-row one is tested in
+# ---------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("rows", FORMS)
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+def test_many_rows_over_the_queries(dim, dtype, rows):
+    """Outputs where the queries are, in one part and in several that are joined."""
+    for lens, cap in (([190, 65], 200), ([5000, 3100], 5056)):
+        cache, model = make(2, 2, dim, cap, dtype), Model(2, 2, dim, dtype)
+        fill(cache, model, lens)
+        gen = torch.Generator().manual_seed(50)
+        q = normal(gen, 2, 70, 4, dim, dtype=dtype).cuda()
+        with form(cache, rows):
+            want = cache.attend(q, ints(lens))
+            assert want.isfinite().all()
+            assert torch.equal(cache.attend(q, ints(lens), out=q), want)
+
+
+@gpu
+@pytest.mark.parametrize("rows", FORMS)
+def test_many_rows_of_hidden_pages_and_bad_sequences(rows):
+    cache, model = make(3, 2, 64, 256, F16, paged=True), Model(3, 2, 64, F16)
+    lens, new = [200, 140, 70], 40
+    fill(cache, model, lens)
+    good = cache.table.clone()
+    gen = torch.Generator().manual_seed(51)
+    q = normal(gen, 3, new, 2, 64, dtype=F16)
+    for bad in (-1, 10 ** 9, cache.k.shape[0]):
+        cache.table.copy_(good)
+        cache.table[0, 1] = bad
+        with form(cache, rows):
+            out = cache.attend(q.cuda(), ints(lens), seq=ints([0, 7, 2])).cpu().double()
+        keep = torch.cat([torch.arange(0, 64), torch.arange(128, 200)])
+        want, bound = attend(q[0], model.held(0, "k")[keep], model.held(0, "v")[keep], 0.125, [keep.numel()] * new, F16)
+        # (the bound's blocks of 64 start at other tokens than the cache's, with at most twice the spread of probabilities)
+        assert ((out[0] - want).abs() <= 2 * bound).all()
+        assert not out[1].any()
+        want, bound = attend(q[2], model.held(2, "k"), model.held(2, "v"), 0.125, [70] * new, F16)
+        assert ((out[2] - want).abs() <= bound).all()
+    cache.table[0] = -1  # nothing is held but the tail
+    with form(cache, rows):
+        out = cache.attend(q.cuda(), ints(lens)).cpu().double()
+    want, bound = attend(q[0], model.held(0, "k")[192:], model.held(0, "v")[192:], 0.125, [8] * new, F16)
+    assert ((out[0] - want).abs() <= bound).all()

@@ -74,7 +74,8 @@ def _check(rc):
 
 class Cache:
     """The cache of one layer: `n_seqs` sequences of up to `max_tokens` tokens (rounded up to whole blocks). With
-    `table` (int32 [n_seqs, blocks], kept, read at every call) sequences take their blocks from a pool of `n_blocks`."""
+    `table` (int32 [n_seqs, blocks], kept, read at every call) sequences take their blocks from a pool of `n_blocks`. Contents of
+    the tensors may be changed in place; the tensors themselves are the cache's for good."""
 
     def __init__(self, n_seqs, n_heads, head_dim, max_tokens, dtype=torch.float16, device="cuda", n_blocks=None, table=None):
         blocks = table.shape[1] if table is not None else -(-int(max_tokens) // BLOCK)
@@ -124,6 +125,13 @@ class Cache:
         self._dev = dev.index
         self._L = load()
         self._ws = {}
+
+    def __setattr__(self, name, value):
+        # calls use the addresses that the cache was made of: another tensor would be ignored, and the old one's memory be
+        # given away under them
+        if name in self.__dict__:
+            raise AttributeError(f"{name} of a cache is fixed: copy into it, or make another with Cache.of")
+        object.__setattr__(self, name, value)
 
     def _index(self, name, x, n):
         if x is None:

@@ -351,3 +351,22 @@ def test_many_rows_of_hidden_pages_and_bad_sequences(rows):
         out = cache.attend(q.cuda(), ints(lens)).cpu().double()
     want, bound = attend(q[0], model.held(0, "k")[192:], model.held(0, "v")[192:], 0.125, [8] * new, F16)
     assert ((out[0] - want).abs() <= bound).all()
+
+
+# ---------------------------------------------------------------------------------------------------
+# the binding
+# ---------------------------------------------------------------------------------------------------
+@gpu
+def test_tensors_of_a_cache_are_fixed():
+    """A cache's tensors change in place alone: another one under the same name would not be read."""
+    cache, model = make(2, 2, 64, 200, F16, paged=True), Model(2, 2, 64, F16)
+    fill(cache, model, [190, 65])
+    for name in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "table"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, getattr(cache, name).clone())
+    with pytest.raises(AttributeError):
+        cache.n_heads = 1
+    cache.table.copy_(cache.table.flip(0))
+    k, _ = cache.read(ints([128, 64]), 64, seq=ints([1, 0]))
+    for s in range(2):
+        assert torch.equal(k[s].cpu(), model.held(s, "k")[:64].float().half()), s

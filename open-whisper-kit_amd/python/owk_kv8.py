@@ -158,8 +158,11 @@ class Cache:
             rows = shape[0]
             if max_new is None:
                 max_new = rows
-        return _BATCH(n, max_new, rows, self._index("lens", lens, n), self._index("seq", seq, n), self._index("off", off, n + 1),
-                      self._index("count", count, n)), n, max_new
+        at = (self._index("lens", lens, n), self._index("seq", seq, n), self._index("off", off, n + 1), self._index("count", count, n))
+        try:
+            return _BATCH(n, max_new, rows, *at), n, max_new
+        except struct.error:
+            raise ValueError(f"max_new {max_new} is out of range") from None
 
     def _rows(self, name, x, shape, heads, dtype):
         s = x.stride()
@@ -204,7 +207,10 @@ class Cache:
             raise ValueError("rows of out lie on each other")
         of = out.dtype
         orow = self._rows("out", out, shape, heads, of if of is torch.float32 else self.dtype)
-        p = _PARAMS(heads, 1 if causal else 0, _TYPES[of], max_len, self.head_dim ** -0.5 if scale is None else scale)
+        try:
+            p = _PARAMS(heads, 1 if causal else 0, _TYPES[of], max_len, self.head_dim ** -0.5 if scale is None else scale)
+        except (struct.error, OverflowError):
+            raise ValueError(f"max_len {max_len} or scale {scale} is out of range") from None
         if q.numel():
             need = self._ws.get((n, max_new, heads, max_len))
             if need is None:  # a function of these sizes alone
@@ -221,6 +227,8 @@ class Cache:
         n = lens.shape[0] if lens.dim() else 0
         if seq is None and n > self.n_seqs:
             raise ValueError(f"{n} entries, and the cache has {self.n_seqs} sequences")
+        if not 0 <= max_tokens < 1 << 31:
+            raise ValueError(f"max_tokens {max_tokens} is out of range")
         h, d = self.n_heads, self.head_dim
         kv = self.k_tail.new_empty((2, n, max_tokens, h, d))
         k, v = kv.unbind(0)

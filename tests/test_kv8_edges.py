@@ -370,3 +370,24 @@ def test_tensors_of_a_cache_are_fixed():
     k, _ = cache.read(ints([128, 64]), 64, seq=ints([1, 0]))
     for s in range(2):
         assert torch.equal(k[s].cpu(), model.held(s, "k")[:64].float().half()), s
+
+
+# ---------------------------------------------------------------------------------------------------
+# arguments out of range
+# ---------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("call", [
+    lambda c, k, i: c.attend(k, i, max_len=1 << 31),
+    lambda c, k, i: c.attend(k, i, max_len=-(1 << 40)),
+    lambda c, k, i: c.attend(k, i, scale=1e60),
+    lambda c, k, i: c.attend(k[0], i[:1], off=i, max_new=1 << 40),
+    lambda c, k, i: c.append(k[0], k[0], i[:1], off=i, max_new=1 << 31),
+    lambda c, k, i: c.append(k, k, i, max_new=-(1 << 33)),
+    lambda c, k, i: c.read(i, -1),
+    lambda c, k, i: c.read(i, (1 << 32) + 1),
+])
+def test_arguments_out_of_range(call):
+    cache = make(2, 2, 64, 128, F16)
+    k, i = torch.zeros((2, 3, 2, 64), dtype=F16, device="cuda"), ints([0, 0])
+    with pytest.raises(ValueError):
+        call(cache, k, i)

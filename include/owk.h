@@ -68,7 +68,8 @@ WHISPER_API int owk_prof_work(struct whisper_context * ctx, const char * kernel_
 WHISPER_API const char * owk_prof_classes(struct whisper_context * ctx);
 
 /* test hooks: intermediates of the last staged call on a state
- * (mel [n_mel][n_len] f32; encoder output [n_audio_ctx][d] f32; cross K/V f16 bits) */
+ * (mel [n_mel][n_len] f32; encoder output [n_audio_ctx][d] f32; cross K/V f16 bits, -1 for a slot or layer that
+ * is not there) */
 WHISPER_API int owk_debug_mel(struct whisper_state * st, float * out, int cap);
 WHISPER_API int owk_debug_enc(struct whisper_context * ctx, struct whisper_state * st, int index, float * out, int cap);
 WHISPER_API int owk_debug_cross(struct whisper_context * ctx, struct whisper_state * st, int slot, int layer,

@@ -584,8 +584,8 @@ void Engine::download_cross(int slot, int layer, uint16_t * kh, uint16_t * vh) c
     OWK_HIP_CHECK(hipStreamSynchronize(stream));
     const int T = n_ctx(), d = hp.n_text_state, H = d / 64;
     const size_t per = (size_t) T * d;
+    if (slot < 0 || slot >= cap_slots || layer < 0 || layer >= hp.n_text_layer) throw std::runtime_error("download_cross: no such slot or layer");
     if (kv8_) {
-        if (slot < 0 || slot >= cap_slots || layer < 0 || layer >= hp.n_text_layer) throw std::runtime_error("download_cross: no such slot");
         const int zl[2] = {flash_attn ? (T + 255) / 256 * 256 : T, slot};  // tokens the slot holds, its sequence
         DevBuf out, idx;
         out.alloc(2 * per * 2);

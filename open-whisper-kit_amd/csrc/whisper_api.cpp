@@ -1219,7 +1219,12 @@ int owk_context_set_kv8(struct whisper_context * ctx, int enable) {
 int owk_debug_cross(struct whisper_context * ctx, struct whisper_state * st, int slot, int layer, uint16_t * k, uint16_t * v) {
     if (!st->eng) return -1;
     const int n = st->eng->n_ctx() * ctx->model->hp.n_text_state;
-    if (k && v) st->eng->download_cross(slot, layer, k, v);
+    try {
+        if (k && v) st->eng->download_cross(slot, layer, k, v);
+    } catch (const std::exception & ex) {
+        log_msg(GGML_LOG_LEVEL_ERROR, "%s: %s\n", __func__, ex.what());
+        return -1;
+    }
     return n;
 }
 

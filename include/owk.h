@@ -36,8 +36,9 @@ WHISPER_API int owk_full_batch(struct whisper_context * ctx, struct whisper_stat
 
 /* hold the decoder's cross-attention keys and values in 8 bits (enable != 0; owk_kv8.h: a scale for each 64 frames and
  * head) instead of f16: half the memory and traffic of what bounds a decode step. Results are close to the f16 ones, not
- * equal. For all states of the context, from their next call on: what a state has encoded before a change is dropped, so
- * not between whisper_encode and whisper_decode, and not while a call runs. Returns 0; -1 for a context made with
+ * equal. For all states of the context, from their next call on: what a state has encoded before a change is dropped (a
+ * whisper_decode fails until the state is encoded again; tokens decoded before stay in its self-attention cache). Not while
+ * a call runs. Returns 0; -1 for a context made with
  * dtw_token_timestamps (which read the f16 attention) or with heads of another size than 64. */
 WHISPER_API int owk_context_set_kv8(struct whisper_context * ctx, int enable);
 

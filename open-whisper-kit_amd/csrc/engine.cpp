@@ -147,7 +147,8 @@ void Engine::set_kv8(bool on) {
     kv8_ = on;
     for (DevBuf * b : {&cross_k_, &cross_v_, &kv8_k_, &kv8_v_, &kv8_ks_, &kv8_vs_, &kv8_kt_, &kv8_vt_, &kv8_fk_, &kv8_fv_, &kv8_ws_})
         b->release();
-    cap_slots = 0;  // the next reserve() allocates the other form
+    cross_slots_ = 0;  // the next reserve() allocates the other form
+    if (cross_ == Cross::held) cross_ = Cross::dropped;
 }
 
 owk_kv8_cache Engine::kv8_cache(int layer) const {
@@ -207,6 +208,10 @@ void Engine::reserve(int slots, int cells) {
     if (slots > cap_slots) {
         sync();
         cap_slots = slots;
+        kv_cells = 0;  // force self-KV re-allocation with the new slot count
+    }
+    if (cross_slots_ != cap_slots) {
+        sync();
         const size_t n = (size_t) hp.n_text_layer * cap_slots * hp.n_audio_ctx * d * 2;
         if (kv8_) {
             const size_t H = hp.n_text_head, blocks = (size_t) hp.n_text_layer * cap_slots * kv8_blocks(hp);
@@ -224,7 +229,7 @@ void Engine::reserve(int slots, int cells) {
             cross_k_.alloc(n);
             cross_v_.alloc(n);
         }
-        kv_cells = 0;  // force self-KV re-allocation with the new slot count
+        cross_slots_ = cap_slots;
     }
     if (cells > kv_cells) {
         sync();
@@ -570,6 +575,7 @@ void Engine::encode(const std::vector<int> & slots, const std::vector<int> & off
         }
     }
     kq_rmul_ = nullptr;
+    cross_ = Cross::held;
 }
 
 void Engine::download_enc(int index, float * host) const {
@@ -585,6 +591,7 @@ void Engine::download_cross(int slot, int layer, uint16_t * kh, uint16_t * vh) c
     const int T = n_ctx(), d = hp.n_text_state, H = d / 64;
     const size_t per = (size_t) T * d;
     if (slot < 0 || slot >= cap_slots || layer < 0 || layer >= hp.n_text_layer) throw std::runtime_error("download_cross: no such slot or layer");
+    if (cross_ == Cross::dropped) throw std::runtime_error("download_cross: dropped by a change of form");
     if (kv8_) {
         const int zl[2] = {flash_attn ? (T + 255) / 256 * 256 : T, slot};  // tokens the slot holds, its sequence
         DevBuf out, idx;
@@ -716,6 +723,7 @@ void Engine::decode(const std::vector<DecodeRow> & rows, const std::vector<int> 
         d_stg_.alloc(st_bytes_);
     }
     if (n_logit_rows > R) throw std::runtime_error("decode: more logit rows than rows");
+    if (cross_ == Cross::dropped) throw std::runtime_error("decode: the encoded audio was dropped when the form of its keys and values changed");
 
     // checks the kernels rely on (fail loudly rather than read out of bounds)
     if ((int64_t) cap_slots * std::max(kv_cells, T) * d >= (int64_t) 1 << 31)

@@ -176,6 +176,8 @@ private:
     // slot storage
     DevBuf cross_k_, cross_v_;   // [L][cap_slots][n_audio_ctx][d]
     bool kv8_ = false;
+    int cross_slots_ = 0;        // slots that the cross K/V were allocated for
+    enum class Cross { none, held, dropped } cross_ = Cross::none;  // encoded, or encoded and released by set_kv8
     DevBuf kv8_k_, kv8_v_;       // kv8_: codes [L][cap_slots][blocks][head][64 * 64], and their scales and tails
     DevBuf kv8_ks_, kv8_vs_, kv8_kt_, kv8_vt_;
     DevBuf kv8_fk_, kv8_fv_;     // one layer's f16 K/V of an encode call [clip][head][n_ctx][64], on their way to codes

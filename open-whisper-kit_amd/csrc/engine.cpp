@@ -536,7 +536,7 @@ void Engine::encode(const std::vector<int> & slots, const std::vector<int> & off
         throw std::runtime_error("encode: cross K/V offsets exceed 32 bits");
     if (kv8_) {
         if (hp.n_text_state != hp.n_text_head * 64) throw std::runtime_error("encode: kv8 needs heads of 64");
-        if (kv8_fk_.bytes < (size_t) M * d * 2) {
+        if (kv8_fk_.bytes < (size_t) M * d * 2 || kv8_fv_.bytes < (size_t) M * d * 2) {
             sync();
             kv8_fk_.alloc((size_t) M * d * 2);
             kv8_fv_.alloc((size_t) M * d * 2);

@@ -112,7 +112,8 @@ WHISPER_API int owk_kv8_read(const struct owk_kv8_cache * cache, int n, int max_
 WHISPER_API void owk_debug_kv8_entry(const struct owk_kv8_cache * cache, const struct owk_kv8_batch * batch, int b,
                                      int64_t out[4]);
 WHISPER_API int64_t owk_debug_kv8_page(const struct owk_kv8_cache * cache, int seq, int i);
-/* test hook: owk_kv8_attend takes its many-row form for calls of more than `rows` rows a key/value head (0: by its own rule) */
+/* test hook: owk_kv8_attend takes its many-row form for calls of more than `rows` rows a key/value head (0: by its own rule).
+ * For the calling thread alone; workspaces that were asked for before are of the other form's size. */
 WHISPER_API void owk_debug_kv8_set_many_rows(int rows);
 
 /* what the calling thread's last failed call found wrong ("" if none failed) */

@@ -5,7 +5,6 @@
 // operand that its matrix product reads along its sum (keys along D, values along the tokens), 16
 // contiguous bytes a lane. The incomplete last block (tail) lies in 16 bits in the same two orders.
 #include <algorithm>
-#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -1208,7 +1207,7 @@ void kv8_read(hipStream_t s, const Kv8Call & call, const int32_t * first, const 
     });
 }
 
-static std::atomic<int> g_many_rows{0};
+static thread_local int g_many_rows = 0;
 void kv8_set_many_rows(int rows) { g_many_rows = rows; }
 
 // How a call is run: host arithmetic on its sizes. The keys are cut into parts of `per` blocks, a workgroup each; entries may
@@ -1221,7 +1220,7 @@ Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len) {
     // take 54 us either way, of 96 rows 77 us in tiles of 16 and 67 in tiles of 128, 4 clips of 300 rows (36k) 35 and 45;
     // at heads of 128, 4 chunks of 80 rows over 4000 keys (10k) 39 and 35, of 132 rows 52 and 42.
     plan.many = rows > 32 && (double) tiles16 * pairs * blocks >= (call.c.head_dim == 64 ? 56000 : 13000);
-    if (const int over = g_many_rows.load()) plan.many = rows > over;
+    if (const int over = g_many_rows) plan.many = rows > over;
     const int mrows = MANY_WAVES * MR * 16;
     const int64_t tiles = plan.many ? (rows + mrows - 1) / mrows : tiles16;
     const int64_t groups = tiles * pairs;

@@ -77,7 +77,7 @@ struct Kv8Plan {
     bool fits = true;          // false: more rows or workgroups than a launch can have
     size_t ws_bytes = 0;
 };
-void kv8_set_many_rows(int rows);  // for tests: calls of more rows a head run in many-row tiles; 0: by kv8_plan's own rule
+void kv8_set_many_rows(int rows);  // for tests, of this thread: calls of more rows a head run in many-row tiles; 0: by kv8_plan's own rule
 Kv8Plan kv8_plan(const Kv8Call & call, int group, int max_len);
 
 void kv8_append(hipStream_t s, const Kv8Call & call, const Kv8Rows & k, const Kv8Rows & v);

@@ -3,12 +3,13 @@ hidden blocks, of values that are not finite, in both forms of attention (16-row
 test_kv8.py's."""
 import contextlib
 import math
+import threading
 
 import pytest
 import torch
 
 import owk_kv8 as KV
-from test_kv8 import BF16, BLOCK, F16, Model, attend, check_attend, fill, ints, make, normal
+from test_kv8 import BF16, BLOCK, F16, Model, Raw, _batch, _desc, _params, attend, check_attend, fill, ints, make, normal
 
 gpu = pytest.mark.gpu
 FORMS = [32, 1 << 30]  # rows of a head above which tiles of 128 rows are taken
@@ -391,3 +392,26 @@ def test_arguments_out_of_range(call):
     k, i = torch.zeros((2, 3, 2, 64), dtype=F16, device="cuda"), ints([0, 0])
     with pytest.raises(ValueError):
         call(cache, k, i)
+
+
+def test_the_switch_of_the_form_is_a_threads_own():
+    """owk_debug_kv8_set_many_rows on one thread changes no other thread's calls."""
+    L = Raw()
+    d, b, p = _desc(n_seqs=1, n_heads=1, n_blocks=4096, max_blocks=4096), _batch(n=1, max_new=40), _params(n_q_heads=1)
+    sizes = []
+
+    def other():
+        sizes.append(L.owk_kv8_attend_workspace(d, b, p))
+
+    want = [L.owk_kv8_attend_workspace(d, b, p)]
+    try:
+        for rows in (32, 1 << 30):
+            KV.load().owk_debug_kv8_set_many_rows(rows)
+            want.append(L.owk_kv8_attend_workspace(d, b, p))
+            t = threading.Thread(target=other)
+            t.start()
+            t.join()
+    finally:
+        KV.load().owk_debug_kv8_set_many_rows(0)
+    assert want[1] != want[2]  # the switch does something here
+    assert sizes == [want[0]] * 2

@@ -28,6 +28,9 @@ __device__ __forceinline__ const char * row_at(const Kv8Call & a, const Kv8Rows 
     return r.p + ((a.b.off ? 0 : (int64_t) b * r.entry) + (e.row0 + i) * r.row + (int64_t) head * r.head) * bytes;
 }
 
+// threadIdx.x & 63, counted anew: not a register that is kept through a loop
+__device__ __forceinline__ int lane_again() { return (int) __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)); }
+
 template <typename T> __device__ __forceinline__ float to_f32(T x) { return (float) x; }
 
 __device__ __forceinline__ float wave_max(float x) {
@@ -342,7 +345,7 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
                                             Acc<D> & acc) {
     typedef T vec8 __attribute__((ext_vector_type(8)));
     constexpr bool BF = !std::is_same<T, _Float16>::value;
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int lane = lane_again(), c = lane & 15, g = lane >> 4;
     // values, dimension-major: lane (c, g) reads keys 16 g .. 16 g + 15 of dimension 16 dt + c
     // (asked for before the scores where the registers allow it)
     auto values = [&](int dt, int k) { return *(const u32x4 *) (vt + (dt * 16 + c) * BLK + 16 * g + 8 * k); };
@@ -1048,19 +1051,29 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
     }
 
     // lane (c, g) holds dimensions 16 d + 4 g .. + 3 of its rows
+    // l is brought to [1/2, 1) by a power of two, so that sums of values near the end of f32 stay in it
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+        const int up = __builtin_amdgcn_frexp_expf(l[r]), fin = (int) sig[r] - 6 - up;
+        m[r] += (float) up;
+        l[r] = __builtin_amdgcn_frexp_mantf(l[r]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[r][d][i] = ldexpf(o[r][d][i], fin);
+    }
     const bool tail = hi > full && mine > full * BLK;
     const int64_t t = ((int64_t) e.seq * a.c.n_heads + head) * BLK * D;
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
-        const int row = row0 + r * 16 + c;
-        const float fin = sig[r] == NONE ? 0.0f : ldexpf(1.0f, (int) sig[r] - 6);
+        const int lane = lane_again(), row = row0 + r * 16 + (lane & 15), dim = 4 * (lane >> 4);
         Acc<D> acc;
         acc.m = m[r];
         acc.l = 0.25f * l[r];
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc.o[d][i] = o[r][d][i] * fin;
+            for (int i = 0; i < 4; ++i) acc.o[d][i] = o[r][d][i];
         if (tail && row0 + r * 16 < nrows) {
             const T * qr = row < nrows ? (const T *) row_at(a, p.q, e, b, row / p.group, head * p.group + row % p.group, 2) : nullptr;
             attend_tail<T, D>((const T *) a.c.k_tail + t, (const T *) a.c.v_tail + t, qr, p.q.vec, unit[r] == unit[r] ? p.scale * LOG2E : NAN,
@@ -1071,14 +1084,14 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
         if (p.splits > 1) {
             const int64_t t16 = (int64_t) tiles * (MROWS / 16);
             float * ws = p.ws + (((((int64_t) b * a.c.n_heads + head) * t16 + row / 16) * p.splits + split) * 16 + row % 16) * (D + 2);
-            if (g == 0) {
+            if (dim == 0) {
                 ws[0] = acc.m;
                 ws[1] = sum;
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) ws[2 + d * 16 + 4 * g + i] = acc.o[d][i];
+                for (int i = 0; i < 4; ++i) ws[2 + d * 16 + dim + i] = acc.o[d][i];
         } else {
             O * out = (O *) row_at(a, p.out, e, b, row / p.group, head * p.group + row % p.group, sizeof(O));
             const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -1089,10 +1102,10 @@ __global__ __launch_bounds__(MW * 64, D == 64 ? 3 : 2) void k_kv8_attend_tiles(K
 #pragma unroll
                 for (int i = 0; i < 4; ++i) y[i] = (O) (sum == 0.0f ? 0.0f : acc.o[d][i] * f);
                 if (p.out.vec) {
-                    *(vec4 *) (out + d * 16 + 4 * g) = y;
+                    *(vec4 *) (out + d * 16 + dim) = y;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) out[d * 16 + 4 * g + i] = y[i];
+                    for (int i = 0; i < 4; ++i) out[d * 16 + dim + i] = y[i];
                 }
             }
         }

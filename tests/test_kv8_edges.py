@@ -80,6 +80,21 @@ def test_nothing_is_seen_of_a_hidden_block(dim, dtype, rows, causal):
     assert ((outs[0][0].cpu().double() - want).abs() <= 2 * bound).all()
 
 
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_near_the_end_of_f32(dim):
+    """Tiles of 128 rows over whole blocks: the sum of a row's weighted values passes the range of f32, the output does not."""
+    gen = torch.Generator().manual_seed(54)
+    n, new = 256, 40
+    v, k = spread(gen, n, 1, dim).abs() * 2.0 ** 125, 0.1 * spread(gen, n, 1, dim)
+    cache, model = one_head(BF16, k, v)
+    q = spread(gen, 1, new, 1, dim).to(BF16)
+    want, bound = attend(q[0], model.held(0, "k"), model.held(0, "v"), dim ** -0.5, [n] * new, torch.float32)
+    with form(cache, 32):
+        got = cache.attend(q.cuda(), ints([n]), out=torch.empty((1, new, 1, dim), device="cuda"))
+    assert ((got[0].cpu().double() - want).abs() <= bound).all()
+
+
 # ---------------------------------------------------------------------------------------------------
 # tails
 # ---------------------------------------------------------------------------------------------------

@@ -401,7 +401,7 @@ __device__ __forceinline__ void attend_tail(const T * kt, const T * vt, const T 
             const int k = t >> 1, e = 4 * (t & 1) + i;
             ph[k][e] = (T) (BF ? p : p * 16384.0f);
             if (BF) pl[k][e] = (T) (p - to_f32(ph[k][e]));
-            ls += BF ? p : to_f32(ph[k][e]);  // what is summed is what multiplies the values
+            ls += BF ? to_f32(ph[k][e]) + to_f32(pl[k][e]) : to_f32(ph[k][e]);  // what is summed is what multiplies the values
         }
     if (!BF) ls *= 1.0f / 16384.0f;
     uint32_t bad = 0;  // of the lane's 16 keys
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
         const float mb = none ? -INFINITY : (float) top * f;
         float alpha;
         const float fb = acc.merge(mb, alpha);
-        float pr[4][4], ls = 0.0f;
+        float pr[4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -618,15 +618,17 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void k_kv8_attend_rows(Kv8
                 for (int i = 0; i < 4; ++i) pr[t][i] = 16 * g + 4 * t + i < here ? pr[t][i] : 0.0f;
         }
         i32x4 ph, pl;
+        int lh = 0, ll = 0;  // what is summed is what multiplies the values: the digits, exactly
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            ls += (pr[t][0] + pr[t][1]) + (pr[t][2] + pr[t][3]);
             int h, l;
             digits(pr[t][0], pr[t][1], pr[t][2], pr[t][3], UNIT, h, l);
             ph[t] = h;
             pl[t] = l;
+            lh = __builtin_amdgcn_sdot4(h, 0x01010101, lh, false);
+            ll = __builtin_amdgcn_sdot4(l, 0x01010101, ll, false);
         }
-        acc.l += none ? 0.0f : fb * ls;
+        acc.l += none ? 0.0f : fb * (1.0f / UNIT) * (float) (lh * 256 + ll);
         const float fo = none ? 0.0f : fb * svl * (1.0f / UNIT);
         if (__any(alpha != 1.0f)) {
 #pragma unroll

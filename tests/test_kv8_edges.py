@@ -95,6 +95,20 @@ def test_values_near_the_end_of_f32(dim):
     assert ((got[0].cpu().double() - want).abs() <= bound).all()
 
 
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, F16), (64, BF16), (128, BF16)])
+@pytest.mark.parametrize("n", [64, 50])
+def test_equal_values(dim, dtype, n):
+    """Weights are divided by their own sum as they were rounded: tokens of equal values give that value to f32's last bits, over
+    a block of codes and over a tail, however few of them a row sees."""
+    gen = torch.Generator().manual_seed(55)
+    k = 0.5 * spread(gen, n, 2, dim)
+    v = torch.full((n, 2, dim), 0.75, dtype=torch.float64)
+    cache, model = one_head(dtype, k, v)
+    check_attend(cache, model, [0], [n], 1, True, scale=0.1, out_type=torch.float32)
+    check_attend(cache, model, [n - 12], [12], 2, True, scale=0.1, out_type=torch.float32)
+
+
 # ---------------------------------------------------------------------------------------------------
 # tails
 # ---------------------------------------------------------------------------------------------------

@@ -72,13 +72,18 @@ LOGIT_RTOL = 1e-3  # of the largest logit: f32 re-association through the layers
 
 
 def _run(w, pcms, **params):
-    """Each clip's logits by the tokens they follow: {(clip, tokens): logits}, from one owk_full_batch call."""
+    """Each clip's logits by the tokens they follow: {(clip, tokens): logits}, from one owk_full_batch call. What is picked is
+    not the model's choice but a draw from the tokens before it (a few tokens far above the rest, unevenly spaced for beams), so
+    that every run meets the same prefixes."""
     states = [w.new_state() for _ in pcms]
     got = {}
 
     def cb(ctx, state, tokens, n_tokens, logits, user):
         key = (states.index(state), tuple(tokens[i].id for i in range(n_tokens)))
-        got.setdefault(key, np.ctypeslib.as_array(logits, shape=(w.n_vocab,)).astype(np.float64))
+        x = np.ctypeslib.as_array(logits, shape=(w.n_vocab,))
+        got.setdefault(key, x.astype(np.float64))
+        rng = np.random.default_rng(key[1])
+        x[rng.choice(np.arange(300, 40000), 8, replace=False)] = x[np.isfinite(x)].max() + 60 - np.cumsum(1 + 3 * rng.random(8))
 
     f = C.CFUNCTYPE(None, C.c_void_p, C.c_void_p, C.POINTER(owk.TokenData), C.c_int, C.POINTER(C.c_float), C.c_void_p)(cb)
     p = w.params(params.pop("strategy", 0), language="en", temperature_inc=0.0, no_timestamps=True, **params)
@@ -107,7 +112,7 @@ def _model(model_path, tmp_path, model):
 @pytest.mark.parametrize("model", ["tiny.en", "l3-mini", "tiny.en q5_0"])
 @pytest.mark.parametrize("beams", [0, 4])
 def test_clips_of_a_batch(model_path, clips, tmp_path, model, beams):
-    """Each clip of a batch has the logits that it has alone, after every prefix that both runs met; and not another clip's.
+    """Each clip of a batch has the logits that it has alone, after every prefix; and not another clip's.
     With quantised weights a batch differs from a clip alone in either form of the cache (activations are rounded to 1/127 of
     their block's largest, so an f32 difference can move one by a step): there a clip's logits have to be nearer to its own than to
     any other clip's, and the 8-bit cache's to the f16 cache's of the same clip."""
@@ -126,8 +131,8 @@ def test_clips_of_a_batch(model_path, clips, tmp_path, model, beams):
         _, batch16 = _run(w16, pcms, **kw)
         w16.close()
     for c, alone in enumerate(runs):
-        both = [t for _, t in alone if (c, t) in batch]
-        assert len(both) >= 4, (c, len(both), len(alone))
+        both = [t for _, t in alone]
+        assert len(both) >= 12 and all((c, t) in batch for t in both), c
         met = 0
         for t in both:
             others = [_apart(batch[o, t], alone[0, t]) for o in range(len(pcms)) if o != c and (o, t) in batch]
@@ -136,8 +141,7 @@ def test_clips_of_a_batch(model_path, clips, tmp_path, model, beams):
             if quant:
                 assert mine < min(others, default=np.inf), (c, t)
                 others16 = [_apart(batch16[o, t], batch[c, t]) for o in range(len(pcms)) if o != c and (o, t) in batch16]
-                if (c, t) in batch16:
-                    assert _apart(batch16[c, t], batch[c, t]) < min(others16, default=np.inf), (c, t)
+                assert _apart(batch16[c, t], batch[c, t]) < min(others16, default=np.inf), (c, t)
             else:
                 assert mine <= LOGIT_RTOL, (c, t, mine)
                 assert min(others, default=np.inf) > 8 * LOGIT_RTOL, (c, t)

@@ -153,7 +153,9 @@ void Engine::set_kv8(bool on) {
 
 owk_kv8_cache Engine::kv8_cache(int layer) const {
     const HParams & hp = m->hp;
-    const size_t H = hp.n_text_head, nb = kv8_blocks(hp), blocks = (size_t) cap_slots * nb * layer, tails = (size_t) cap_slots * layer * H * kKv8Block * 64;
+    const size_t H = hp.n_text_head, nb = kv8_blocks(hp), blocks = (size_t) cap_slots * nb * layer;
+    // with flash_attn a tail is complete once the pad rows follow its layer's own: one layer's tails serve all
+    const size_t tails = flash_attn ? 0 : (size_t) cap_slots * layer * H * kKv8Block * 64;
     owk_kv8_cache c{};
     c.device = m->device;
     c.dtype = OWK_KV8_F16;
@@ -215,7 +217,7 @@ void Engine::reserve(int slots, int cells) {
         const size_t n = (size_t) hp.n_text_layer * cap_slots * hp.n_audio_ctx * d * 2;
         if (kv8_) {
             const size_t H = hp.n_text_head, blocks = (size_t) hp.n_text_layer * cap_slots * kv8_blocks(hp);
-            const size_t tails = (size_t) hp.n_text_layer * cap_slots * H * kKv8Block * 64 * 2;
+            const size_t tails = (flash_attn ? 1 : (size_t) hp.n_text_layer) * cap_slots * H * kKv8Block * 64 * 2;
             for (DevBuf * b : {&kv8_k_, &kv8_v_}) b->alloc(blocks * H * kKv8Block * 64);
             for (DevBuf * b : {&kv8_ks_, &kv8_vs_}) {
                 b->alloc(blocks * H * 4);

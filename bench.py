@@ -205,6 +205,8 @@ def parse(argv=None):
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-prof", action="store_true", help="disable per-class HIP-event timing")
     ap.add_argument("--verbose", action="store_true")
+    ap.add_argument("--kv8", action="store_true", help="cross keys and values in 8 bits (owk_context_set_kv8); not the default "
+                    "workload, whose numerics are the reference's")
     return ap.parse_args(argv)
 
 
@@ -293,7 +295,7 @@ class GpuRunner:
         if L.owk_device_ok(local) != 1:
             raise RuntimeError("libwhisper.so: no usable gfx950 device / code object")
         owk.quiet()
-        self.w = w = owk.Whisper(self.model_path, device=local)
+        self.w = w = owk.Whisper(self.model_path, device=local, kv8=args.kv8)
         B = args.batch
         # clips of this rank, resident in HBM for the timed region
         self.host = [S.synth_audio(CLIP_SAMPLES, seed) for seed in clip_seeds(rank, B)]
@@ -479,10 +481,11 @@ def main(argv=None, runner=None):
         raise RuntimeError(f"fixed-work violation: tokens per clip {sorted(set(ntok))}")
 
     roof = None
+    profiled = args.model + ("+kv8" if args.kv8 else "")  # the committed profiles are the f16 cache's
     classes = run.profile() if not args.no_prof else {}
     if classes:
         top = sorted(classes, key=lambda c: -classes[c]["ms"])[:TOP_CLASSES]
-        rd = rocprof_dominant(classes, args.model)  # also time the committed profile's dominant class
+        rd = rocprof_dominant(classes, profiled)  # also time the committed profile's dominant class
         if rd and rd not in top:
             top.append(rd)
         alone = {}
@@ -492,7 +495,9 @@ def main(argv=None, runner=None):
                 continue
             v = dict(got[c])
             alone[c] = v
-        roof = roofline(classes, 1e3 * dt / args.steps, alone or None, args.model)
+        roof = roofline(classes, 1e3 * dt / args.steps, alone or None, profiled)
+        if args.kv8 and roof["kernel_class"] == "attn_cross":
+            roof["kernel"] = "owk::k_kv8_attend_rows (k_kv8.hip)"
         if rank == 0:
             for c, v in alone.items():
                 log(f"[bench] alone {c:16s} {v['ms']:10.2f} ms  launches {v['launches']:7d}  "
@@ -518,11 +523,11 @@ def main(argv=None, runner=None):
         "higher_is_better": True,
         "scaling": "weak",
         "vs_baseline": None,
-        "dtype": DTYPE[kind],
+        "dtype": DTYPE[kind] + (", cross K/V int8" if args.kv8 else ""),
         "data": "synthetic: seeded 30 s 16 kHz clips; random-init weights of the named architecture",
         "config": {"workload": f"{args.model} {kind.upper()} weights, {B} x 30 s clips per GPU per step, greedy "
                                f"(temperature_inc=0), no_timestamps, EOT suppressed, {MAX_TOKENS + 1} "
-                               f"tokens/clip, audio resident in HBM",
+                               f"tokens/clip, audio resident in HBM" + (", cross K/V in 8 bits" if args.kv8 else ""),
                    "model": args.model, "clips_per_gpu": B, "global_batch": world * B,
                    "tokens_per_clip": MAX_TOKENS + 1, "parallelism": f"clip-sharded x{world} (no collectives)"},
         "roofline": roof,

@@ -5,7 +5,9 @@
  * head and for keys and values apart, 64 * head_dim signed codes and one scale s = max|x| / 127 (f32):
  * a code c = rint(x / s) stands for c * s. The last, incomplete block of a sequence (its tail) stays in
  * the 16-bit type it came in until its 64 tokens are there, so what a token is rounded to depends on
- * the data alone and never on how many tokens a call brought. A block with a value that is not finite
+ * the data alone and never on how many tokens a call brought. (What is attended does depend on it: tokens are
+ * seen as the cache holds them when the call runs, so the tokens of a chunk that completes a block see
+ * codes where tokens that came one by one saw 16 bits.) A block with a value that is not finite
  * reads as NaN throughout (keys or values of that head).
  *
  * All pointers are device memory of `device`; every call is queued on `stream` (a hipStream_t, NULL =
@@ -92,7 +94,21 @@ struct owk_kv8_attend_params {
 };
 
 /* out = softmax(scale * q . k) . v for each row and query head; zeros for a row that sees nothing. Rows
- * behind an entry's own are left as they were. Sums, maxima and the accumulators are f32. */
+ * behind an entry's own are left as they were. out may lie where q lies (the same type and strides); other
+ * overlaps are not allowed.
+ *
+ * Scores, sums, maxima and the accumulators are f32, and a weight is divided by the sum of the weights as they
+ * were rounded. What is multiplied has fewer bits, also where out is f32:
+ *   calls of few rows   each query element to 2^-16 of its row's largest, each weight to 2^-16 of the largest of its
+ *                       block of 64 tokens
+ *   calls of many rows  weights to half precision (2^-11 of each, or 2^-15 of its block's largest if that is more); bf16
+ *                       query elements below 2^-14 of their row's largest to 2^-25 of it
+ *   tails, in both      queries, keys and values as they are; weights to half precision (f16), 2^-16 of each (bf16)
+ * Which form a call takes follows from its sizes (rows, heads, entries, length), not from its data.
+ *
+ * A row whose query is not finite is NaN if it sees anything; so is a row that sees any of a block that is not finite, or
+ * a tail token with a value that is not finite (a tail key that is not finite counts by its score). Hidden tokens and
+ * blocks add nothing, whatever they hold. A row whose weighted values add up beyond the range of f32 may be infinite. */
 WHISPER_API int owk_kv8_attend(const struct owk_kv8_cache * cache, const struct owk_kv8_batch * batch,
                                const struct owk_kv8_attend_params * params, const struct owk_kv8_rows * q,
                                const struct owk_kv8_rows * out, void * workspace, size_t workspace_bytes, void * stream);

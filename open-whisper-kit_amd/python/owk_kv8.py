@@ -189,8 +189,9 @@ class Cache:
     def attend(self, q, lens, seq=None, off=None, count=None, max_new=None, max_len=0, scale=None, causal=False, out=None):
         """softmax(scale * q . k) . v over what the sequences hold: tokens [0, lens[b]), or with causal, for row i,
         [0, lens[b] + i] (its own tokens appended before). scale None: 1 / sqrt(head_dim). `max_len`: no sequence holds
-        more (a hint for splitting the work). `out`: a tensor like q, or float32; rows that are no entry's stay as they are (undefined in a new
-        tensor). No gradients."""
+        more (a hint for splitting the work). `out`: a tensor like q (q itself, too), or float32; rows that are no entry's stay as they are
+        (undefined in a new tensor). Weights and some queries have fewer bits than 32, also into float32: owk_kv8.h says how many. No
+        gradients."""
         shape = q.shape
         b, n, max_new = self._batch(shape, lens, seq, off, count, max_new)
         heads = shape[-2]
